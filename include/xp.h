@@ -531,6 +531,127 @@ int xp_moe_layer(const uint16_t* x, int64_t T, int64_t H, const void* topk_ids,
                  int64_t work_bytes, uint16_t* out, int activation,
                  void* stream);
 
+/* ---- Router: the choice of experts, the balance loss, their gradient ----
+ * No counterpart in the reference, which takes topk_ids and topk_weights from
+ * vLLM (experts.py:380-400).
+ * Logits: T rows of E (row_stride elements apart, consecutive within a row),
+ * of type XP_FLOAT32, XP_BFLOAT16 or XP_FLOAT16. A logit that is NaN or -inf
+ * is masked: its expert has probability 0 and is never chosen. mask
+ * (nullable, uint8[T]): tokens with 0 are padding; their ids are -1, their
+ * weights 0, and they count nowhere. Everything that is summed is summed in
+ * 32 bits or more. E is at most XP_MAX_EXPERTS, topk at most 64. */
+#define XP_FLOAT32 0
+#define XP_BFLOAT16 1
+#define XP_FLOAT16 2
+#define XP_SCORE_SOFTMAX 0
+#define XP_SCORE_SIGMOID 1
+
+/* ids[T][topk] (int32): the topk best experts of each token in descending
+ * order, equal ones by the lower index; -1 where fewer are left. weights
+ * (fp32): score * scale, the score being the softmax over all experts or the
+ * sigmoid, over the sum of the chosen scores if renormalize. bias (nullable,
+ * fp32[E]) is added to the scores for the choice alone, in 64 bits. groups >
+ * 1 (at most 64, dividing E, E at most 1024): only the topk_groups groups of
+ * E / groups consecutive experts with the largest best score (with a bias:
+ * the largest sum of two best) are chosen from. */
+int xp_router_choose(const void* logits, int dtype, int64_t T, int64_t E,
+                     int64_t row_stride, int64_t topk, int scoring,
+                     int renormalize, const float* bias, int64_t groups,
+                     int64_t topk_groups, double scale, const uint8_t* mask,
+                     float* weights, int32_t* ids, void* stream);
+
+/* Bytes of the workspace of the two calls below (no initial contents). */
+int64_t xp_router_workspace_bytes(int64_t T, int64_t E, int64_t num_seqs);
+
+/* Balance loss of a given choice topk_ids[T][topk]. seq_offsets (nullable,
+ * int32[num_seqs + 1], ascending): the rows of sequence s are [seq_offsets[s],
+ * seq_offsets[s + 1]), rows outside all of them are padding; null (num_seqs
+ * 1): all rows are one sequence. counts[num_seqs][E] (int32) receives how
+ * often each expert is chosen (ids outside [0, E) count nowhere),
+ * tokens[num_seqs + 1] (int32) the valid tokens of each sequence and then the
+ * number of sequences that have any, and *loss (fp32, device) the mean over
+ * those of sum_e f_e P_e, f_e = E counts_e / (topk tokens) and P_e the mean
+ * probability of e (the softmax, or the sigmoid over its sum). */
+int xp_router_balance(const void* logits, int dtype, int64_t T, int64_t E,
+                      int64_t row_stride, int64_t topk, int scoring,
+                      const void* topk_ids, int topk_elem_bytes,
+                      const uint8_t* mask, const int32_t* seq_offsets,
+                      int64_t num_seqs, void* work, int64_t work_bytes,
+                      int32_t* counts, int32_t* tokens, float* loss,
+                      void* stream);
+
+/* xp_router_choose and xp_router_balance of its choice in one pass over the
+ * logits. Rows outside every sequence get ids -1 and weights 0. */
+int xp_router_choose_balance(const void* logits, int dtype, int64_t T,
+                             int64_t E, int64_t row_stride, int64_t topk,
+                             int scoring, int renormalize, const float* bias,
+                             int64_t groups, int64_t topk_groups, double scale,
+                             const uint8_t* mask, const int32_t* seq_offsets,
+                             int64_t num_seqs, float* weights, int32_t* ids,
+                             void* work, int64_t work_bytes, int32_t* counts,
+                             int32_t* tokens, float* loss, void* stream);
+
+/* The gradient by the logits, grad[T][E] (their type, rows consecutive):
+ * through the weights (grad_weights fp32[T][topk] and the ids, nullable) and
+ * through the loss (counts and tokens as written above and grad_loss, an fp32
+ * scalar on the device, nullable together). The choice, the counts and the
+ * bias have no gradient. Rows of padding get zeros. */
+int xp_router_backward(const void* logits, int dtype, int64_t T, int64_t E,
+                       int64_t row_stride, int64_t topk, int scoring,
+                       int renormalize, double scale, const uint8_t* mask,
+                       const int32_t* seq_offsets, int64_t num_seqs,
+                       const void* topk_ids, int topk_elem_bytes,
+                       const float* grad_weights, const int32_t* counts,
+                       const int32_t* tokens, const float* grad_loss,
+                       void* grad, void* stream);
+
+/* ---- Low-rank adapters beside the experts' projections ----
+ * No counterpart in the reference. The adapters of a projection of S slices
+ * (2 for gate and up) of n columns from K inputs, for L adapters and E
+ * experts, bf16 or fp16, R = the storage rank:
+ *   a [L][E][S][R][Kp]   Kp = K rounded up to 32, zeros behind K and behind
+ *                        an adapter's rank
+ *   b [L][E][S][np][R]   np = n rounded up to 16, zeros likewise
+ *   scales [L] (fp32), ranks [L] (int32, 0 .. R: what is read of a and b)
+ * R is 16, 32, 64, 96 or 128; K and n are multiples of 8.
+ */
+#define XP_LORA_MAX_RANK 128
+
+/* Bytes of the workspace of the calls below for npairs pairs (no initial
+ * contents; 256-byte aligned). adapters * experts is at most 2^20 - 1. */
+int64_t xp_lora_workspace_bytes(int64_t npairs, int64_t adapters,
+                                int64_t experts);
+
+/* Lists the pairs p = t * topk + k of each (adapter, expert) in the
+ * workspace: adapter adapter_ids[t], expert topk_ids[p] (null: expert 0). A
+ * pair whose adapter or expert is out of range has none. expert_map (nullable,
+ * int32[experts]): only pairs whose expert has a slot in [0, slots) are
+ * listed at all. One launch. */
+int xp_lora_group(const void* adapter_ids, int adapter_elem_bytes,
+                  const void* topk_ids, int topk_elem_bytes, int64_t T,
+                  int64_t topk, const int32_t* expert_map, int64_t slots,
+                  int64_t adapters, int64_t experts, void* work,
+                  int64_t work_bytes, void* stream);
+
+/* out[p][s n + c] = base[p][s n + c] + scales[l] * sum_r b[l][e][s][c][r] *
+ * (sum_k a[l][e][s][r][k] x[row][k]) for every listed pair p of adapter l and
+ * expert e, row = t, or p with per_pair; one rounding to the type of out. A
+ * pair without an adapter gets base. base null: 0. Rows are x_stride,
+ * base_stride and out_stride elements apart (multiples of 8); out may be
+ * base. Sums and the inner product in fp32 (the inner product enters the
+ * second one as a sum of two values of the type). grouped != 0: the workspace
+ * holds the listing of xp_lora_group for the same ids and sizes; else the call
+ * makes it. Calls of at most 64 pairs group themselves and need no workspace. */
+int xp_lora_apply(const void* x, int dtype, int64_t x_stride, int per_pair,
+                  int64_t T, int64_t topk, int64_t K, const void* a,
+                  const void* b, const float* scales, const int32_t* ranks,
+                  int64_t adapters, int64_t experts, int64_t slices, int64_t n,
+                  int64_t R, const void* adapter_ids, int adapter_elem_bytes,
+                  const void* topk_ids, int topk_elem_bytes,
+                  const int32_t* expert_map, int64_t slots, const void* base,
+                  int64_t base_stride, void* out, int64_t out_stride,
+                  void* work, int64_t work_bytes, int grouped, void* stream);
+
 /* ---- measurement ---- */
 
 /* Reads `count` records of record_bytes (a multiple of 4096) at the given

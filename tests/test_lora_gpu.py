@@ -1,0 +1,275 @@
+"""GPU parity of the low-rank adapters (csrc/lora.hip) against the products in 64 bits.
+
+Tolerance, per value, with U = 2^-24 and h = half a step of the type (bf16
+2^-8, fp16 2^-11, relative): the inner product u_r is an fp32 sum of K products
+of which each carries at most K roundings, |du_r| <= 2 K U sum_k |A x| (the
+matrix unit's sums are taken to lose up to twice an fp32 add's rounding); u
+enters the second product as two values of the type, losing h^2 of it (bf16
+2^-16); that product adds 2 R U of its terms' magnitude. The result is rounded
+once: h of itself. All magnitudes are taken from sum |B| (|A| |x|).
+"""
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
+HALF = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}
+TINY = {torch.bfloat16: 2.0**-133, torch.float16: 2.0**-25}  # half the least step
+
+
+def _lora():
+    from vllm_expert_pager import lora
+
+    return lora
+
+
+def _stack(L, E, K, n, ranks, slices, dtype, max_rank, seed, scale=1.7):
+    """A loaded stack, its matrices per adapter, and the scales."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    stack = _lora().LowRankAdapters(L, E, K, slices * n, max_rank, slices=slices, dtype=dtype)
+    mats = []
+    for i in range(L):
+        r = ranks[i % len(ranks)]
+        if r == 0:
+            mats.append(None)
+            continue
+        a = (torch.randn((E, slices, r, K), generator=g, device="cuda") / K**0.5).to(dtype)
+        b = (0.5 * torch.randn((E, slices, n, r), generator=g, device="cuda")).to(dtype)
+        stack.load(i, a, b, scale / (i + 1))
+        mats.append((a, b, np.float32(scale / (i + 1))))
+    return stack, mats
+
+
+def _ref(x, mats, adapter, ids, slices, n, K, base, per_pair, dtype):
+    """(value, bound) in 64 bits."""
+    T = adapter.numel()
+    k = 1 if ids is None else ids.shape[1]
+    P = T * k
+    out = torch.zeros((P, slices * n), dtype=torch.float64, device="cuda") if base is None else base.double()
+    mag = torch.zeros_like(out)
+    h = HALF[dtype]
+    for p in range(P):
+        a, e = int(adapter[p // k]), 0 if ids is None else int(ids.reshape(-1)[p])
+        if not 0 <= a < len(mats) or mats[a] is None or not 0 <= e < mats[a][0].shape[0]:
+            continue
+        ma, mb, sc = mats[a]
+        xr = x[p if per_pair else p // k].double()
+        r = ma.shape[2]
+        for s in range(slices):
+            A, B = ma[e, s].double(), mb[e, s].double()
+            out[p, s * n : (s + 1) * n] += float(sc) * (B @ (A @ xr))
+            mag[p, s * n : (s + 1) * n] += abs(float(sc)) * (2 * (K + r) * U + h * h) * (B.abs() @ (A.abs() @ xr.abs()))
+    return out, mag + 4 * U * out.abs() + h * 1.01 * out.abs() + TINY[dtype]
+
+
+CASES = [
+    # T, E, topk, K, n, slices, ranks, max_rank, L, dtype, per_pair, with base
+    (1, 1, 1, 8, 8, 1, [1], 1, 1, torch.bfloat16, False, False),
+    (1, 16, 8, 256, 128, 2, [16], 16, 3, torch.bfloat16, False, False),
+    (5, 1, 1, 40, 24, 1, [4, 7], 8, 2, torch.float16, False, True),
+    (64, 1, 1, 264, 136, 1, [16, 0, 64, 33], 64, 5, torch.float16, False, True),
+    (65, 1, 1, 264, 136, 1, [16, 0, 64, 33], 64, 5, torch.bfloat16, False, True),
+    (8, 64, 8, 512, 256, 1, [32, 5], 32, 4, torch.bfloat16, True, False),
+    (40, 8, 3, 384, 120, 2, [96, 70], 96, 3, torch.bfloat16, False, True),
+    (200, 4, 2, 136, 512, 1, [128, 100, 1], 128, 3, torch.float16, True, False),
+    (300, 1, 1, 1000, 72, 3, [12], 12, 1, torch.bfloat16, False, False),
+    (130, 256, 4, 128, 64, 1, [8], 8, 20, torch.bfloat16, False, False),
+    (17, 4, 4, 2048, 2048, 2, [64], 64, 2, torch.bfloat16, False, True),
+]
+
+
+@pytest.mark.parametrize("T, E, topk, K, n, slices, ranks, max_rank, L, dtype, per_pair, with_base", CASES)
+@pytest.mark.parametrize("wide", [torch.int32, torch.int64])
+def test_against_the_products(T, E, topk, K, n, slices, ranks, max_rank, L, dtype, per_pair, with_base, wide):
+    g = torch.Generator(device="cuda").manual_seed(T + K)
+    stack, mats = _stack(L, E, K, n, ranks, slices, dtype, max_rank, 5)
+    P = T * topk
+    x = torch.randn((P if per_pair else T, K), generator=g, device="cuda").to(dtype)
+    base = torch.randn((P, slices * n), generator=g, device="cuda").to(dtype) if with_base else None
+    adapter = torch.randint(-2, L + 1, (T,), generator=g, device="cuda").to(wide)  # some of them out of range
+    adapter[0] = 0
+    ids = None
+    if E > 1:
+        ids = torch.rand((T, E), generator=g, device="cuda").argsort(1)[:, :topk].to(wide)
+        ids[0, 0] = 0
+        if T > 3:
+            ids[1, 0], ids[2, 0] = -1, E
+            ids[3] = 1  # the same expert several times
+    got = _lora().low_rank(x, stack, adapter, ids, base=base)
+    ref, bound = _ref(x, mats, adapter, ids, slices, n, K, base, per_pair, dtype)
+    assert got.dtype == dtype and tuple(got.shape) == (P, slices * n)
+    err = (got.double() - ref).abs()
+    assert (err <= bound).all(), float((err / bound).max())
+    # Pairs without an adapter: base as it was, or zeros.
+    k = topk
+    none = torch.tensor([not 0 <= int(adapter[p // k]) < L or (ids is not None and not 0 <= int(ids.reshape(-1)[p]) < E)
+                         for p in range(P)], device="cuda")
+    assert torch.equal(got[none], base[none] if base is not None else torch.zeros_like(got[none]))
+
+
+def test_many_groups_and_pairs_of_one():
+    """A prefill over thousands of groups (some of them with many tiles), against a second call pair by pair."""
+    lora = _lora()
+    g = torch.Generator(device="cuda").manual_seed(0)
+    L, E, K, n, T, topk = 20, 256, 128, 64, 900, 4
+    stack, _ = _stack(L, E, K, n, [16, 3], 1, torch.bfloat16, 16, 1)
+    x = torch.randn((T, K), generator=g, device="cuda").to(torch.bfloat16)
+    adapter = torch.randint(-1, L, (T,), generator=g, device="cuda")
+    adapter[::3] = 7
+    ids = torch.rand((T, E), generator=g, device="cuda").argsort(1)[:, :topk].to(torch.int32)
+    ids[::2, 0] = 11
+    whole = lora.low_rank(x, stack, adapter, ids)
+    parts = [lora.low_rank(x[t : t + 16], stack, adapter[t : t + 16], ids[t : t + 16]) for t in range(0, T, 16)]
+    assert torch.equal(whole, torch.cat(parts))  # a pair's result does not depend on the others
+    assert torch.equal(whole, lora.low_rank(x, stack, adapter, ids))
+
+
+@pytest.mark.parametrize("T", [3, 200])
+def test_in_place_strides_and_rows_behind(T):
+    """out = base in place, rows apart in every tensor, and the rows behind them left as they were."""
+    lora = _lora()
+    g = torch.Generator(device="cuda").manual_seed(2)
+    stack, _ = _stack(3, 1, 64, 40, [8], 1, torch.bfloat16, 8, 3)
+    wide = torch.randn((T + 2, 96), generator=g, device="cuda").to(torch.bfloat16)
+    x = wide[1 : T + 1, 16:80]
+    y = torch.randn((T + 2, 56), generator=g, device="cuda").to(torch.bfloat16)
+    before = y.clone()
+    adapter = torch.randint(-1, 3, (T,), generator=g, device="cuda").to(torch.int32)
+    want = lora.low_rank(x.contiguous(), stack, adapter, base=y[1 : T + 1, 8:48].contiguous())
+    out = lora.low_rank(x, stack, adapter, base=y[1 : T + 1, 8:48], out=y[1 : T + 1, 8:48])
+    assert torch.equal(out, want) and out.data_ptr() == y[1:, 8:].data_ptr()
+    before[1 : T + 1, 8:48] = want
+    assert torch.equal(y, before)
+
+
+def test_loading_and_clearing():
+    """A place that is loaded again with a smaller rank holds nothing of the old adapter; a cleared one adds nothing."""
+    lora = _lora()
+    g = torch.Generator(device="cuda").manual_seed(4)
+    stack = lora.LowRankAdapters(2, 3, 72, 48, 40, slices=2)
+    fresh = lora.LowRankAdapters(2, 3, 72, 48, 40, slices=2)
+    big = [torch.randn(s, generator=g, device="cuda") for s in ((3, 2, 40, 72), (3, 2, 24, 40))]
+    small = [torch.randn(s, generator=g, device="cuda") for s in ((3, 2, 3, 72), (3, 2, 24, 3))]
+    stack.load(1, *big, 2.0)
+    stack.load(1, *small, 0.5)
+    fresh.load(1, *small, 0.5)
+    for name in ("a", "b", "scales", "ranks"):
+        assert torch.equal(getattr(stack, name), getattr(fresh, name))
+    x = torch.randn((5, 72), generator=g, device="cuda").to(torch.bfloat16)
+    ids = torch.tensor([[0, 1], [2, 1], [0, 2], [1, 0], [2, 0]], device="cuda")
+    who = torch.ones((5,), dtype=torch.int32, device="cuda")
+    assert lora.low_rank(x, stack, who, ids).abs().sum() > 0
+    stack.clear(1)
+    assert (lora.low_rank(x, stack, who, ids) == 0).all()
+    assert (lora.low_rank(x, stack, who - 1, ids) == 0).all()  # never loaded
+    one = lora.LowRankAdapters(1, 1, 72, 24, 8)
+    one.load(0, torch.ones((4, 72)), torch.ones((24, 4)))  # without the experts' and slices' dimensions, from the host
+    assert (lora.low_rank(torch.ones_like(x), one, who - 1) == 288).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_extreme_values(dtype):
+    """Infinite and NaN tokens stay in their rows, and unused ranks and columns add nothing to them; huge and tiny
+    inner products keep their precision in fp16."""
+    lora = _lora()
+    stack = lora.LowRankAdapters(1, 1, 40, 8, 5, dtype=dtype)
+    a, b = torch.ones((5, 40)), torch.ones((8, 5))
+    stack.load(0, a, b, 1.0)
+    x = torch.ones((70, 40), dtype=dtype, device="cuda")
+    x[1, 39] = float("inf")
+    x[2, 0] = float("nan")
+    x[3] = 60000.0  # u = 2.4e6, beyond fp16; the result is infinite there
+    x[4] = 2.0**-24
+    who = torch.zeros((70,), dtype=torch.int32, device="cuda")
+    y = lora.low_rank(x, stack, who)
+    assert (y[0] == 200).all() and (y[5:] == 200).all()
+    assert torch.isinf(y[1]).all() and torch.isnan(y[2]).all()
+    want = (x[3, 0].double() * 200).to(dtype)
+    assert torch.equal(y[3], want.expand(8))
+    assert torch.equal(y[4], torch.full((8,), 200 * 2.0**-24, dtype=torch.float64, device="cuda").to(dtype))
+    stack.load(0, a, b, 2.0**-12)  # u beyond fp16, the result inside it: no overflow on the way
+    y = lora.low_rank(x, stack, who)
+    want = (x[3, 0].double() * 200 * 2.0**-12).to(dtype)
+    assert torch.equal(y[3], want.expand(8))
+
+
+def test_no_tokens():
+    lora = _lora()
+    stack = lora.LowRankAdapters(2, 4, 16, 16, 4)
+    x = torch.empty((0, 16), dtype=torch.bfloat16, device="cuda")
+    ids = torch.empty((0, 2), dtype=torch.int32, device="cuda")
+    assert tuple(lora.low_rank(x, stack, ids[:, 0].contiguous(), ids).shape) == (0, 16)
+
+
+@pytest.mark.parametrize("T", [4, 100])
+def test_graph_and_stream(T):
+    """Captured and replayed on changed tokens, adapters and experts; a call on a side stream."""
+    lora = _lora()
+    g = torch.Generator(device="cuda").manual_seed(6)
+    stack, _ = _stack(4, 16, 128, 64, [16, 7], 2, torch.bfloat16, 16, 9)
+    sets = []
+    for _ in range(3):
+        x = torch.randn((T, 128), generator=g, device="cuda").to(torch.bfloat16)
+        who = torch.randint(-1, 4, (T,), generator=g, device="cuda")
+        ids = torch.rand((T, 16), generator=g, device="cuda").argsort(1)[:, :2].contiguous()
+        sets.append((x, who, ids, lora.low_rank(x, stack, who, ids)))
+    buf = [t.clone() for t in sets[0][:3]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = lora.low_rank(buf[0], stack, buf[1], buf[2])
+    for i in (1, 2, 0, 1):
+        for d, s in zip(buf, sets[i]):
+            d.copy_(s)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, sets[i][3])
+        lora.low_rank(sets[0][0], stack, sets[0][1], sets[0][2]).sum().item()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = lora.low_rank(*sets[2][:1], stack, *sets[2][1:3])
+    side.synchronize()
+    assert torch.equal(y, sets[2][3])
+
+
+def test_refusals():
+    lora = _lora()
+    for bad in (dict(max_rank=129), dict(max_rank=0), dict(in_features=12), dict(out_features=20), dict(adapters=0),
+                dict(adapters=1 << 12, experts=1 << 8), dict(slices=3), dict(dtype=torch.float32)):
+        how = {**dict(adapters=2, experts=4, in_features=16, out_features=32, max_rank=8), **bad}
+        with pytest.raises(ValueError):
+            lora.LowRankAdapters(**how)
+    s = lora.LowRankAdapters(2, 4, 16, 32, 8)
+    for a, b in (((4, 1, 9, 16), (4, 1, 32, 9)), ((4, 1, 4, 16), (4, 1, 32, 5)), ((3, 1, 4, 16), (4, 1, 32, 4)),
+                 ((4, 1, 4, 8), (4, 1, 32, 4))):
+        with pytest.raises(ValueError):
+            s.load(0, torch.zeros(a), torch.zeros(b))
+    with pytest.raises(ValueError):
+        s.load(2, torch.zeros((4, 1, 4, 16)), torch.zeros((4, 1, 32, 4)))
+    with pytest.raises(ValueError):
+        s.clear(-1)
+    x = torch.zeros((3, 16), dtype=torch.bfloat16, device="cuda")
+    who = torch.zeros((3,), dtype=torch.int32, device="cuda")
+    ids = torch.zeros((3, 2), dtype=torch.int32, device="cuda")
+    bad = [
+        lambda: lora.low_rank(x, s, who),  # four experts, no ids
+        lambda: lora.low_rank(x[:2], s, who, ids),
+        lambda: lora.low_rank(x.half(), s, who, ids),
+        lambda: lora.low_rank(x.cpu(), s, who, ids),
+        lambda: lora.low_rank(x, s, who.cpu(), ids),
+        lambda: lora.low_rank(x, s, who.float(), ids),
+        lambda: lora.low_rank(x, s, who, ids[:2]),
+        lambda: lora.low_rank(x, s, who[:, None], ids),
+        lambda: lora.low_rank(x.t().contiguous().t(), s, who, ids),
+        lambda: lora.low_rank(x, s, who, ids, base=torch.zeros((5, 32), dtype=torch.bfloat16, device="cuda")),
+        lambda: lora.low_rank(x, s, who, ids, out=torch.zeros((6, 32), device="cuda")),
+        lambda: lora.low_rank(torch.zeros((3, 20), dtype=torch.bfloat16, device="cuda")[:, :16], s, who, ids),
+        lambda: lora.low_rank(torch.zeros((3, 24), dtype=torch.bfloat16, device="cuda")[:, 4:20], s, who, ids),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was taken")

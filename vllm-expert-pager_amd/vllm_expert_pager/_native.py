@@ -89,6 +89,7 @@ class XpDecodeScale(ctypes.Structure):
 _P = c_ptr
 _I = ctypes.c_int
 _L = c_i64
+_D = ctypes.c_double
 _SIGNATURES = {
     "xp_last_error": (ctypes.c_char_p, []),
     "xp_version": (ctypes.c_char_p, []),
@@ -141,6 +142,16 @@ _SIGNATURES = {
     "xp_encode_workspace_bytes": (_L, [_L, _L, _L]),
     "xp_encode_rows_split": (_I, [_P, _L, _L, _L, _L, _P, _L, _P, _L, _P, _P, _L, _P]),
     "xp_moe_topk_sum": (_I, [_P, _L, _L, _L, _P, _I, _L, _P, _P]),
+    "xp_router_choose": (_I, [_P, _I, _L, _L, _L, _L, _I, _I, _P, _L, _L, _D, _P, _P, _P, _P]),
+    "xp_router_workspace_bytes": (_L, [_L, _L, _L]),
+    "xp_router_balance": (_I, [_P, _I, _L, _L, _L, _L, _I, _P, _I, _P, _P, _L, _P, _L, _P, _P, _P, _P]),
+    "xp_router_choose_balance": (_I, [_P, _I, _L, _L, _L, _L, _I, _I, _P, _L, _L, _D, _P, _P, _L, _P, _P, _P, _L, _P, _P,
+                                      _P, _P]),
+    "xp_router_backward": (_I, [_P, _I, _L, _L, _L, _L, _I, _I, _D, _P, _P, _L, _P, _I, _P, _P, _P, _P, _P, _P]),
+    "xp_lora_workspace_bytes": (_L, [_L, _L, _L]),
+    "xp_lora_group": (_I, [_P, _I, _P, _I, _L, _L, _P, _L, _L, _L, _P, _L, _P]),
+    "xp_lora_apply": (_I, [_P, _I, _L, _I, _L, _L, _L, _P, _P, _P, _P, _L, _L, _L, _L, _L, _P, _I, _P, _I, _P, _L, _P,
+                           _L, _P, _L, _P, _L, _I, _P]),
 }
 
 _lib = None
@@ -190,6 +201,20 @@ def call(name: str, *args) -> None:
 def stream() -> int:
     """Raw hipStream_t of torch's current stream."""
     return torch.cuda.current_stream().cuda_stream
+
+
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """``call`` with the current stream of t's device as the last argument, that device being the current one."""
+    if t.device.index == torch.cuda.current_device():
+        check(getattr(lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
+        return
+    with torch.cuda.device(t.device):
+        check(getattr(lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
+
+
+def require_same_device(t: torch.Tensor, other: torch.Tensor, what: str) -> None:
+    if t.device != other.device:
+        raise ValueError(f"{what} must be on {other.device} (got {t.device})")
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
