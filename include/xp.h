@@ -460,6 +460,25 @@ int xp_moe_experts_part(const uint8_t* xq, const float* xs, int64_t T,
                         const int32_t* tiles, void* work, int64_t work_bytes,
                         uint16_t* out, int activation, void* stream);
 
+/* xp_moe_experts_part one launch at a time, with terms of the pairs' own, for
+ * low-rank adapters beside the experts (xp_lora_apply). stage 1: gate and up,
+ *   gate = bf16(h[:I] + add_gate_up[pair][:I]), up likewise from [I:2I],
+ * leaving the bf16 activations [T*topk][I] at the start of `work` as well, from
+ * which the caller makes add_down. stage 2: down, on the same `work`,
+ *   out[pair] = bf16(topk_weight[pair] * (w2 . a + add_down[pair])).
+ * add_gate_up is bf16 [T*topk][2I], add_down bf16 [T*topk][H], 16-byte aligned;
+ * either may be null (none). Both calls take the same other arguments; a pair
+ * whose terms are zero gets the bits of xp_moe_experts. */
+int xp_moe_experts_add(const uint8_t* xq, const float* xs, int64_t T,
+                       int64_t topk, const float* topk_weight, int64_t H,
+                       int64_t I, const uint8_t* w13, const float* w13_scale,
+                       const uint8_t* w2, const float* w2_scale, int64_t slots,
+                       int64_t num_experts, const int32_t* offsets,
+                       const int32_t* pairs, const int32_t* tiles, void* work,
+                       int64_t work_bytes, const uint16_t* add_gate_up,
+                       const uint16_t* add_down, uint16_t* out, int activation,
+                       int stage, void* stream);
+
 /* Workspace bytes xp_moe_experts_noalloc holds per device (32 MiB: a
  * 2048-token top-8 prefill at I = 512 needs 27.5 MB). */
 #define XP_MOE_SCRATCH_BYTES (32LL << 20)

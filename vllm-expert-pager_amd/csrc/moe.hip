@@ -44,6 +44,7 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kBM = 64;          // pairs per tile
@@ -763,20 +764,58 @@ __device__ __forceinline__ AOffsets a_offsets(const int* s_row, int64_t lda, int
   return o;
 }
 
+// Four bf16 terms of a lane's four columns, added to its sums.
+__device__ __forceinline__ void add_terms(f32x4& acc, const u32x2& t) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) acc[r] += bf16_value((t[r >> 1] >> (16 * (r & 1))) & 0xffffu);
+}
+
+// The pairs' gate and up terms, columns col .. col + 3 and I + col .. of row
+// 16 mi + j, four subtiles' loads in flight at a time.
+template <int MI>
+__device__ __forceinline__ void add_gate_up(f32x4 (&acc)[MI][2], const uint16_t* __restrict__ add, const int* s_pair,
+                                            int64_t col, int64_t I) {
+  constexpr int kBatch = 4;
+  const int j = threadIdx.x & 15;
+#pragma unroll
+  for (int m0 = 0; m0 < MI; m0 += kBatch) {
+    u32x2 t[kBatch][2];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (m0 + i >= MI) continue;
+      const int p = s_pair[16 * (m0 + i) + j];
+      const uint16_t* src = add + static_cast<int64_t>(p < 0 ? 0 : p) * 2 * I + col;
+      t[i][0] = *reinterpret_cast<const u32x2*>(src);
+      t[i][1] = *reinterpret_cast<const u32x2*>(src + I);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (m0 + i >= MI) continue;
+      add_terms(acc[m0 + i][0], t[i][0]);
+      add_terms(acc[m0 + i][1], t[i][1]);
+    }
+  }
+}
+
 // GEMM1 at prefill sizes: gate and up for 128 activation columns of a wide
 // tile per item; each wave owns 16 columns (16 gate and 16 up rows) and runs
 // the K blocks in order, so a column's value does not depend on the
 // workgroup width or the tile height. Then a = bf16(bf16(silu(bf16 gate)) *
 // bf16 up) is quantised to fp8 per row over the workgroup's 128 columns, one
 // scale group. Only the 16-row subtiles that hold pairs are multiplied.
-template <int ACT, bool STREAM>
+//
+// ADD: the pairs' own terms (add[pair][2I], bf16: gate columns, then up) are
+// added to the sums before they are rounded, and the bf16 activations are kept
+// (work.a16) beside the fp8 ones: low-rank adapters beside the experts.
+template <int ACT, bool ADD, bool STREAM>
 __global__ void __launch_bounds__(kGemmWaves * 64) gemm1_kernel(const uint8_t* __restrict__ xq,
                                                                const float* __restrict__ xs, int64_t H, int64_t I,
                                                                int topk, const uint8_t* __restrict__ w13,
                                                                const float* __restrict__ w13_scale,
                                                                const int32_t* __restrict__ pairs,
                                                                const int32_t* __restrict__ wide, int64_t wmax,
-                                                               int64_t npairs, Work work) {
+                                                               int64_t npairs, Work work,
+                                                               const uint16_t* __restrict__ add) {
   constexpr int NW = kGemmWaves, NT = NW * 64, NC = NW * 16;
   constexpr int NB = 2 * NC;       // weight rows per item: per wave 16 gate, then 16 up
   static_assert(NC == kKB, "a workgroup covers one 128-column scale group of the activations");
@@ -947,6 +986,10 @@ __global__ void __launch_bounds__(kGemmWaves * 64) gemm1_kernel(const uint8_t* _
       // the rule gemm2_narrow_kernel applies, on the same bf16 values). The
       // fp8 rows are staged in the A stage of the last step, which no load
       // targets before the next item's first step writes them out.
+      const int64_t own_col = static_cast<int64_t>(cur.col) * NC + 16 * wave + 4 * q;
+      if constexpr (ADD) {
+        if (add) add_gate_up<MI>(acc, add, s_pair[cb], own_col, I);
+      }
 #pragma unroll
       for (int mi = 0; mi < MI; ++mi) {
         float m = 0.f;
@@ -958,6 +1001,12 @@ __global__ void __launch_bounds__(kGemmWaves * 64) gemm1_kernel(const uint8_t* _
         }
         m = quad16_max(m);
         if (q == 0) s_m[wave][16 * mi + j] = m;
+        if constexpr (ADD) {
+          const int p = s_pair[cb][16 * mi + j];
+          const u32x2 w = {bf16_bits(acc[mi][0][0]) | bf16_bits(acc[mi][0][1]) << 16,
+                           bf16_bits(acc[mi][0][2]) | bf16_bits(acc[mi][0][3]) << 16};
+          if (p >= 0) *reinterpret_cast<u32x2*>(work.a16 + static_cast<int64_t>(p) * I + own_col) = w;
+        }
       }
       lds_barrier();  // s_m; and every wave is done with the last stage
       if (tid < 16 * MI) {
@@ -1054,7 +1103,7 @@ __device__ __forceinline__ void subtile_rows(const Tile& tile, int r0, const int
 // (subtile, column block) items.
 constexpr int kSplitRound = 16;  // K blocks per round, kSplitRound / 4 per wave
 
-template <int ACT>
+template <int ACT, bool ADD>
 __global__ void __launch_bounds__(kThreads) gemm1_narrow_kernel(const uint8_t* __restrict__ xq,
                                                                 const float* __restrict__ xs, int64_t H, int64_t I,
                                                                 int topk, const uint8_t* __restrict__ w13,
@@ -1062,7 +1111,7 @@ __global__ void __launch_bounds__(kThreads) gemm1_narrow_kernel(const uint8_t* _
                                                                 const int32_t* __restrict__ offsets,
                                                                 const int32_t* __restrict__ pairs,
                                                                 const int32_t* __restrict__ tiles, int nsub,
-                                                                Work work) {
+                                                                Work work, const uint16_t* __restrict__ add) {
   constexpr int kPerWave = kSplitRound / (kThreads / 64);
   __shared__ int s_row[16];
   __shared__ int s_pair[16];
@@ -1137,6 +1186,17 @@ __global__ void __launch_bounds__(kThreads) gemm1_narrow_kernel(const uint8_t* _
   }
 
   if (wave == 0) {
+    if constexpr (ADD) {
+      if (add) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int p = s_pair[4 * q + r];
+          const uint16_t* src = add + static_cast<int64_t>(p < 0 ? 0 : p) * 2 * I + c0 + j;
+          acc[0][r] += bf16_value(src[0]);
+          acc[1][r] += bf16_value(src[I]);
+        }
+      }
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float a = act_and_mul<ACT>(bf16_round(acc[0][r]), bf16_round(acc[1][r]));
@@ -1695,7 +1755,7 @@ __global__ void __launch_bounds__(kThreads) gemm2_decode_kernel(
 // rounding as gemm2_kernel.
 constexpr int kQuantK = 2048;  // activation columns quantised per LDS round
 
-template <int CH>
+template <int CH, bool ADD>
 __global__ void __launch_bounds__(kThreads) gemm2_narrow_kernel(int64_t H, int64_t I,
                                                                 const float* __restrict__ topk_weight,
                                                                 const uint8_t* __restrict__ w2,
@@ -1703,7 +1763,8 @@ __global__ void __launch_bounds__(kThreads) gemm2_narrow_kernel(int64_t H, int64
                                                                 const int32_t* __restrict__ offsets,
                                                                 const int32_t* __restrict__ pairs,
                                                                 const int32_t* __restrict__ tiles, int nsub,
-                                                                Work work, uint16_t* __restrict__ out) {
+                                                                Work work, uint16_t* __restrict__ out,
+                                                                const uint16_t* __restrict__ add) {
   constexpr int kRoundKB = kQuantK / kKB;
   __shared__ int s_row[16];
   __shared__ int s_pair[16];
@@ -1781,6 +1842,15 @@ __global__ void __launch_bounds__(kThreads) gemm2_narrow_kernel(int64_t H, int64
     __syncthreads();  // the next round rewrites s_act
   }
 
+  if constexpr (ADD) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int p = s_pair[4 * q + r];
+      const uint16_t* src = add + static_cast<int64_t>(p < 0 ? 0 : p) * H + n0 + 32 * wave + j;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) acc[t][r] += bf16_value(src[16 * t]);
+    }
+  }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int row = 4 * q + r;
@@ -1803,14 +1873,17 @@ __global__ void __launch_bounds__(kThreads) gemm2_narrow_kernel(int64_t H, int64
 // waves owns 16 TB columns and runs the K blocks in order over the tile's
 // fp8 activations; persistent over items through the operand ring as
 // gemm1_kernel.
-template <int TB, bool STREAM>
+//
+// ADD: add[pair][H] (bf16) is added to the sums before the routed weight.
+template <int TB, bool ADD, bool STREAM>
 __global__ void __launch_bounds__(kGemmWaves * 64) gemm2_kernel(int64_t H, int64_t I,
                                                                const float* __restrict__ topk_weight,
                                                                const uint8_t* __restrict__ w2,
                                                                const float* __restrict__ w2_scale,
                                                                const int32_t* __restrict__ pairs,
                                                                const int32_t* __restrict__ wide, int64_t wmax,
-                                                               int64_t npairs, Work work, uint16_t* __restrict__ out) {
+                                                               int64_t npairs, Work work, uint16_t* __restrict__ out,
+                                                               const uint16_t* __restrict__ add) {
   constexpr int NW = kGemmWaves, NT = NW * 64, NC = NW * 16 * TB;  // output columns per item
   constexpr int kStageRows = 64;  // output rows staged per epilogue round: 64 x NC bf16 = one weight stage
   static_assert(kStageRows * NC * 2 == NC * kRowB, "an epilogue round fills one weight stage");
@@ -1964,6 +2037,28 @@ __global__ void __launch_bounds__(kGemmWaves * 64) gemm2_kernel(int64_t H, int64
         st = st == kRing - 1 ? 0 : st + 1;
       }
 
+      if constexpr (ADD) {
+        constexpr int kBatch = 4;  // subtiles whose terms are in flight together
+#pragma unroll
+        for (int m0 = 0; m0 < MI; m0 += kBatch) {
+          u32x2 term[kBatch][TB];
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            if (m0 + i >= MI) continue;
+            const int p = s_pair[cb][16 * (m0 + i) + j];
+            const uint16_t* src =
+                add + static_cast<int64_t>(p < 0 ? 0 : p) * H + n0 + 16 * TB * wave + 4 * q;
+#pragma unroll
+            for (int t = 0; t < TB; ++t) term[i][t] = *reinterpret_cast<const u32x2*>(src + 16 * t);
+          }
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            if (m0 + i >= MI) continue;
+#pragma unroll
+            for (int t = 0; t < TB; ++t) add_terms(acc[m0 + i][t], term[i][t]);
+          }
+        }
+      }
       // bf16(acc x routed weight), staged 64 rows at a time in the weight
       // stage of the last step (no load targets it before the next item's
       // first step); the last round is written out at that step.
@@ -2203,10 +2298,17 @@ int cus_per_xcd(int* out) {
   return XP_OK;
 }
 
+// The GEMM launches of one expert call; an expert call of pairs with terms of
+// their own (low-rank adapters) makes them one at a time.
+enum Stage { kGateUp = 1, kDown = 2 };
+
 // The two (or, for few pairs, narrow) GEMM launches of one expert call over a
 // workspace of xp_moe_workspace_bytes(T * topk, I) bytes at `work`.
-// num_experts: the experts that the T * topk pairs are spread over.
-int launch_experts(const uint8_t* xq, const float* xs, int64_t T, int64_t topk, const float* topk_weight, int64_t H,
+// num_experts: the experts that the T * topk pairs are spread over. ADD: the
+// launches of `stages` with the pairs' terms add1 (gate and up; nullable) and
+// add2 (down; nullable).
+template <bool ADD>
+int launch_stages(int stages, const uint16_t* add1, const uint16_t* add2, const uint8_t* xq, const float* xs, int64_t T, int64_t topk, const float* topk_weight, int64_t H,
                    int64_t I, const uint8_t* w13, const float* w13_scale, const uint8_t* w2, const float* w2_scale,
                    int64_t slots, int64_t num_experts, const int32_t* offsets, const int32_t* pairs,
                    const int32_t* tiles, uint8_t* work, uint16_t* out, int act, void* stream) {
@@ -2234,20 +2336,26 @@ int launch_experts(const uint8_t* xq, const float* xs, int64_t T, int64_t topk, 
     // One workgroup per CU: the operand ring takes most of its LDS.
     const int64_t n1 = std::min<int64_t>(per_xcd, per_xcd_tiles * (I / (16 * kGemmWaves)));
     const bool stream_w = stream_weights(npairs, num_experts);
-    auto* gemm1 = act == XP_ACT_GELU
-                      ? (stream_w ? gemm1_kernel<XP_ACT_GELU, true> : gemm1_kernel<XP_ACT_GELU, false>)
-                      : (stream_w ? gemm1_kernel<XP_ACT_SILU, true> : gemm1_kernel<XP_ACT_SILU, false>);
-    hipLaunchKernelGGL(gemm1, dim3(static_cast<unsigned>(8 * n1)), dim3(64 * kGemmWaves), 0, as_stream(stream), xq, xs,
-                       H, I, static_cast<int>(topk), w13, w13_scale, pairs, wide, wmax, npairs, w);
-    rc = check_launch("gemm1_kernel");
-    if (rc) return rc;
+    if (stages & kGateUp) {
+      auto* gemm1 = act == XP_ACT_GELU
+                        ? (stream_w ? gemm1_kernel<XP_ACT_GELU, ADD, true> : gemm1_kernel<XP_ACT_GELU, ADD, false>)
+                        : (stream_w ? gemm1_kernel<XP_ACT_SILU, ADD, true> : gemm1_kernel<XP_ACT_SILU, ADD, false>);
+      hipLaunchKernelGGL(gemm1, dim3(static_cast<unsigned>(8 * n1)), dim3(64 * kGemmWaves), 0, as_stream(stream), xq,
+                         xs, H, I, static_cast<int>(topk), w13, w13_scale, pairs, wide, wmax, npairs, w, add1);
+      rc = check_launch("gemm1_kernel");
+      if (rc || !(stages & kDown)) return rc;
+    }
     // 256 output columns per item where H allows, else 128.
     const int tb = H % (2 * kBN) == 0 ? 2 : 1;
     const int64_t n2 = std::min<int64_t>(per_xcd, per_xcd_tiles * (H / (tb * kBN)));
-    auto* gemm2 = tb == 2 ? (stream_w ? gemm2_kernel<2, true> : gemm2_kernel<2, false>)
-                          : (stream_w ? gemm2_kernel<1, true> : gemm2_kernel<1, false>);
+    auto pick2 = [&](auto add_c) {
+      constexpr bool A = decltype(add_c)::value;
+      return tb == 2 ? (stream_w ? gemm2_kernel<2, A, true> : gemm2_kernel<2, A, false>)
+                     : (stream_w ? gemm2_kernel<1, A, true> : gemm2_kernel<1, A, false>);
+    };
+    auto* gemm2 = ADD && add2 ? pick2(std::integral_constant<bool, ADD>{}) : pick2(std::false_type{});
     hipLaunchKernelGGL(gemm2, dim3(static_cast<unsigned>(8 * n2)), dim3(64 * kGemmWaves), 0, as_stream(stream), H, I,
-                       topk_weight, w2, w2_scale, pairs, wide, wmax, npairs, w, out);
+                       topk_weight, w2, w2_scale, pairs, wide, wmax, npairs, w, out, add2);
     return check_launch("gemm2_kernel");
   }
   const int64_t tiles8 = (bound + 7) / 8 * 8;  // the XCD-aware grids cover whole groups of 8 tiles
@@ -2257,19 +2365,25 @@ int launch_experts(const uint8_t* xq, const float* xs, int64_t T, int64_t topk, 
   // Few pairs: 16-row subtiles x 16 columns, the K blocks split over 4 waves.
   const int64_t g1n = tiles8 * nsub * (I / 16);
   XP_REQUIRE(g1n <= INT32_MAX && nsub * g2 <= INT32_MAX, "xp_moe_experts: grid too large");
-  if (act == XP_ACT_GELU)
-    hipLaunchKernelGGL(gemm1_narrow_kernel<XP_ACT_GELU>, dim3(static_cast<unsigned>(g1n)), dim3(kThreads), 0,
-                       as_stream(stream), xq, xs, H, I, static_cast<int>(topk), w13, w13_scale, offsets, pairs, tiles,
-                       nsub, w);
-  else
-    hipLaunchKernelGGL(gemm1_narrow_kernel<XP_ACT_SILU>, dim3(static_cast<unsigned>(g1n)), dim3(kThreads), 0,
-                       as_stream(stream), xq, xs, H, I, static_cast<int>(topk), w13, w13_scale, offsets, pairs, tiles,
-                       nsub, w);
-  rc = check_launch("gemm1_narrow_kernel");
-  if (rc) return rc;
-  hipLaunchKernelGGL(gemm2_narrow_kernel<kNarrowChunk>, dim3(static_cast<unsigned>(nsub * g2)), dim3(kThreads), 0,
-                     as_stream(stream), H, I, topk_weight, w2, w2_scale, offsets, pairs, tiles, nsub, w, out);
+  if (stages & kGateUp) {
+    auto* gemm1 = act == XP_ACT_GELU ? gemm1_narrow_kernel<XP_ACT_GELU, ADD> : gemm1_narrow_kernel<XP_ACT_SILU, ADD>;
+    hipLaunchKernelGGL(gemm1, dim3(static_cast<unsigned>(g1n)), dim3(kThreads), 0, as_stream(stream), xq, xs, H, I,
+                       static_cast<int>(topk), w13, w13_scale, offsets, pairs, tiles, nsub, w, add1);
+    rc = check_launch("gemm1_narrow_kernel");
+    if (rc || !(stages & kDown)) return rc;
+  }
+  auto* gemm2 = ADD && add2 ? gemm2_narrow_kernel<kNarrowChunk, ADD> : gemm2_narrow_kernel<kNarrowChunk, false>;
+  hipLaunchKernelGGL(gemm2, dim3(static_cast<unsigned>(nsub * g2)), dim3(kThreads), 0, as_stream(stream), H, I,
+                     topk_weight, w2, w2_scale, offsets, pairs, tiles, nsub, w, out, add2);
   return check_launch("gemm2_narrow_kernel");
+}
+
+int launch_experts(const uint8_t* xq, const float* xs, int64_t T, int64_t topk, const float* topk_weight, int64_t H,
+                   int64_t I, const uint8_t* w13, const float* w13_scale, const uint8_t* w2, const float* w2_scale,
+                   int64_t slots, int64_t num_experts, const int32_t* offsets, const int32_t* pairs,
+                   const int32_t* tiles, uint8_t* work, uint16_t* out, int act, void* stream) {
+  return launch_stages<false>(kGateUp | kDown, nullptr, nullptr, xq, xs, T, topk, topk_weight, H, I, w13, w13_scale, w2,
+                              w2_scale, slots, num_experts, offsets, pairs, tiles, work, out, act, stream);
 }
 
 int launch_topk_sum(const uint16_t* contrib, int64_t T, int64_t topk, int64_t H, const void* ids, int eb,
@@ -2378,6 +2492,28 @@ int xp_moe_experts_part(const uint8_t* xq, const float* xs, int64_t T, int64_t t
              (long long)need);
   return launch_experts(xq, xs, T, topk, topk_weight, H, I, w13, w13_scale, w2, w2_scale, slots, num_experts, offsets,
                         pairs, tiles, static_cast<uint8_t*>(work), out, activation, stream);
+}
+
+int xp_moe_experts_add(const uint8_t* xq, const float* xs, int64_t T, int64_t topk, const float* topk_weight, int64_t H,
+                       int64_t I, const uint8_t* w13, const float* w13_scale, const uint8_t* w2, const float* w2_scale,
+                       int64_t slots, int64_t num_experts, const int32_t* offsets, const int32_t* pairs,
+                       const int32_t* tiles, void* work, int64_t work_bytes, const uint16_t* add_gate_up,
+                       const uint16_t* add_down, uint16_t* out, int activation, int stage, void* stream) {
+  const char* what = "xp_moe_experts_add";
+  int rc = check_experts(what, xq, xs, T, topk, topk_weight, H, I, w13, w13_scale, w2, w2_scale, slots, offsets, pairs,
+                         tiles, out, activation);
+  if (rc) return rc;
+  XP_REQUIRE(stage == kGateUp || stage == kDown, "%s: stage %d (1: gate and up, 2: down)", what, stage);
+  XP_REQUIRE(num_experts >= 1 && num_experts <= INT32_MAX, "%s: %lld experts", what, (long long)num_experts);
+  if (T == 0) return XP_OK;
+  XP_REQUIRE(aligned16(add_gate_up) && aligned16(add_down), "%s: the terms must be 16-byte aligned", what);
+  XP_REQUIRE(work && (reinterpret_cast<uintptr_t>(work) & 255) == 0,
+             "%s: the workspace must be non-null and 256-byte aligned", what);
+  const int64_t need = xp_moe_workspace_bytes(T * topk, I);
+  XP_REQUIRE(work_bytes >= need, "%s: workspace of %lld B, needs %lld", what, (long long)work_bytes, (long long)need);
+  return launch_stages<true>(stage, add_gate_up, add_down, xq, xs, T, topk, topk_weight, H, I, w13, w13_scale, w2,
+                             w2_scale, slots, num_experts, offsets, pairs, tiles, static_cast<uint8_t*>(work), out,
+                             activation, stream);
 }
 
 int xp_moe_experts(const uint8_t* xq, const float* xs, int64_t T, int64_t topk, const float* topk_weight, int64_t H,

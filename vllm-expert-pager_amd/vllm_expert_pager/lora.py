@@ -108,6 +108,75 @@ class ExpertAdapters:
     gate_up: LowRankAdapters | None = None
     down: LowRankAdapters | None = None
 
+    def check(self, hidden: int, intermediate: int, experts: int, device: torch.device) -> None:
+        """ValueError unless the stacks fit an expert layer of these sizes."""
+        for stack, what, shape in ((self.gate_up, "gate_up", (experts, 2, hidden, intermediate)),
+                                   (self.down, "down", (experts, 1, intermediate, hidden))):
+            if stack is None:
+                continue
+            have = (stack.experts, stack.slices, stack.in_features, stack.columns)
+            if have != shape or stack.dtype != torch.bfloat16 or stack.device != device:
+                raise ValueError(f"{what} adapters of (experts, slices, inputs, columns) {have} in {stack.dtype} on "
+                                 f"{stack.device} do not fit a layer of {shape} in torch.bfloat16 on {device}")
+        if self.gate_up is not None and self.down is not None and self.gate_up.adapters != self.down.adapters:
+            raise ValueError(f"{self.gate_up.adapters} gate_up and {self.down.adapters} down adapters")
+
+
+@dataclass
+class AdaptedBatch:
+    """A batch's pairs with their adapters, as ``moe.run_experts`` takes them.
+
+    ``gate_up`` holds the pairs' gate and up terms ``(T * topk, 2I)``, made
+    once per layer call: they depend on tokens and ids alone, so the experts
+    may then run in any number of chunks. ``listing`` is the pairs by adapter
+    and expert, shared by both projections of a call in one piece.
+    """
+
+    adapters: ExpertAdapters
+    adapter_ids: torch.Tensor
+    topk_ids: torch.Tensor
+    gate_up: torch.Tensor | None
+    listing: torch.Tensor | None
+
+    def down(self, acts: torch.Tensor, expert_map: torch.Tensor | None, slots: int) -> torch.Tensor | None:
+        """The down projection's terms ``(T * topk, H)`` of the pairs whose expert ``expert_map`` places in a slot
+        (None: all), from their activations ``(T * topk, I)``; the other rows are left unwritten."""
+        stack = self.adapters.down
+        if stack is None:
+            return None
+        T, topk = self.topk_ids.shape
+        out = torch.empty((T * topk, stack.out_features), dtype=stack.dtype, device=acts.device)
+        listing = self.listing
+        if expert_map is not None:
+            listing = group(stack, self.adapter_ids, self.topk_ids, expert_map, slots)
+        apply(acts, stack, self.adapter_ids, self.topk_ids, T, topk, True, None, out, expert_map=expert_map, slots=slots,
+              listing=listing)
+        return out
+
+
+def adapt(x: torch.Tensor, adapters: ExpertAdapters, adapter_ids: torch.Tensor, topk_ids: torch.Tensor,
+          intermediate: int, experts: int) -> AdaptedBatch:
+    """The adapters' part of a layer call that its tokens ``x`` ``(T, H)`` decide, before any expert runs."""
+    nat.require_device(x, "x")
+    if x.dtype != torch.bfloat16 or x.dim() != 2:
+        raise ValueError(f"x must be a 2-D bfloat16 tensor, got {x.dtype} {tuple(x.shape)}")
+    T, H = x.shape
+    adapters.check(H, intermediate, experts, x.device)
+    adapter_ids, topk_ids = _ids(adapter_ids, "adapter_ids", x), _ids(topk_ids, "topk_ids", x)
+    if tuple(adapter_ids.shape) != (T,) or topk_ids.dim() != 2 or topk_ids.shape[0] != T:
+        raise ValueError(f"adapter_ids must be ({T},) and topk_ids ({T}, topk), got {tuple(adapter_ids.shape)} and "
+                         f"{tuple(topk_ids.shape)}")
+    some = adapters.gate_up if adapters.gate_up is not None else adapters.down
+    if some is None or T == 0:
+        return AdaptedBatch(adapters, adapter_ids, topk_ids, None, None)
+    listing = group(some, adapter_ids, topk_ids, None, 0)
+    terms = None
+    if adapters.gate_up is not None:
+        terms = torch.empty((topk_ids.numel(), 2 * intermediate), dtype=x.dtype, device=x.device)
+        apply(x.contiguous(), adapters.gate_up, adapter_ids, topk_ids, T, topk_ids.shape[1], False, None, terms,
+              listing=listing)
+    return AdaptedBatch(adapters, adapter_ids, topk_ids, terms, listing)
+
 
 def _ids(t: torch.Tensor, what: str, like: torch.Tensor) -> torch.Tensor:
     nat.require_same_device(t, like, what)

@@ -26,6 +26,7 @@ from dataclasses import dataclass
 import torch
 
 from vllm_expert_pager import _native as nat
+from vllm_expert_pager import lora
 
 BLOCK = 128  # quantisation group and weight scale block
 MAX_SLOTS = 1024  # slots one route call can address
@@ -181,6 +182,8 @@ def run_experts(
     routing: Routing,
     contrib: torch.Tensor,
     activation: str = "silu",
+    adapted: lora.AdaptedBatch | None = None,
+    expert_map: torch.Tensor | None = None,
 ) -> None:
     """Write ``contrib[t*topk + k]`` (bf16, ``(T*topk, H)``) for every routed pair.
 
@@ -188,7 +191,10 @@ def run_experts(
     ``(S, H, I)``, scales ``(S, 2I/128, H/128)`` and ``(S, H/128, I/128)``
     fp32. Rows of pairs that were not routed are left as they are.
     ``activation`` ("silu" or "gelu") is applied to the gate before the
-    product with up.
+    product with up. ``adapted`` (``lora.adapt`` of the same call) adds the
+    requests' low-rank adapters to the three projections, each term rounded to
+    bf16; ``expert_map``, the one that was routed by, tells a chunk's pairs
+    from the others, which it may leave out.
     """
     act = activation_code(activation)
     T, H = xq.shape
@@ -204,6 +210,23 @@ def run_experts(
         raise ValueError(f"contrib must be contiguous bfloat16 {(T * topk, H)}")
     nbytes = int(nat.lib().xp_moe_workspace_bytes(T * topk, I))
     work = torch.empty((max(nbytes, 1),), dtype=torch.uint8, device=xq.device)
+    if adapted is not None and T > 0:
+        if tuple(adapted.topk_ids.shape) != (T, topk):
+            raise ValueError(f"adapted batch of {tuple(adapted.topk_ids.shape)} ids for ({T}, {topk}) weights")
+        adapted.adapters.check(H, I, routing.experts or routing.slots, xq.device)
+        down = None
+        for stage in (1, 2):  # gate and up, then the adapters on their activations, then down
+            nat.call(
+                "xp_moe_experts_add", _fp8_ptr(xq, "xq"), _f32(xs, "xs").data_ptr(), T, topk, tw.data_ptr(), H, I,
+                _fp8_ptr(w13, "w13"), _f32(w13_scale, "w13_scale").data_ptr(), _fp8_ptr(w2, "w2"),
+                _f32(w2_scale, "w2_scale").data_ptr(), routing.slots, routing.experts or routing.slots,
+                routing.offsets.data_ptr(), routing.pairs.data_ptr(), routing.tiles.data_ptr(), work.data_ptr(), nbytes,
+                nat.ptr(adapted.gate_up), nat.ptr(down), contrib.data_ptr(), act, stage, nat.stream(),
+            )
+            if stage == 1:
+                acts = work[: T * topk * I * 2].view(torch.bfloat16).view(T * topk, I)
+                down = adapted.down(acts, expert_map, routing.slots)
+        return
     nat.call(
         "xp_moe_experts_part", _fp8_ptr(xq, "xq"), _f32(xs, "xs").data_ptr(), T, topk, tw.data_ptr(), H, I,
         _fp8_ptr(w13, "w13"), _f32(w13_scale, "w13_scale").data_ptr(), _fp8_ptr(w2, "w2"),
@@ -344,15 +367,24 @@ def fused_moe(
     expert_map: torch.Tensor | None = None,
     num_experts: int | None = None,
     activation: str = "silu",
+    adapters: lora.ExpertAdapters | None = None,
+    adapter_ids: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """One-shot MoE over a slab: quantise, route, experts, combine.
 
     Without ``expert_map`` the slab holds every expert (slot e = expert e).
-    Pairs whose expert has no slot contribute nothing.
+    Pairs whose expert has no slot contribute nothing. ``adapters`` add the
+    low-rank adapters of the requests, token t's being ``adapter_ids[t]`` (-1:
+    none; such a token gets the bits of a call without adapters).
     """
     S = w13.shape[0]
     E = num_experts if num_experts is not None else (expert_map.numel() if expert_map is not None else S)
     listed = E if expert_map is None else min(E, expert_map.numel())
+    if (adapters is None) != (adapter_ids is None):
+        raise ValueError("adapters and adapter_ids go together")
+    if adapters is not None:
+        return _adapted_layer(x, topk_weights, topk_ids, w13, w13_scale, w2, w2_scale, expert_map, E, activation,
+                              adapters, adapter_ids)
     if topk_weights.dim() == 2 and topk_ids.shape == topk_weights.shape and listed > 0 and S > 0:
         # One native call with one workspace, against seven launches of the
         # separate calls: no identity map, no zero fill of the contributions
@@ -368,6 +400,25 @@ def fused_moe(
     contrib = torch.zeros((T * topk, x.shape[1]), dtype=torch.bfloat16, device=x.device)
     run_experts(xq, xs, topk_weights, w13, w13_scale, w2, w2_scale, r, contrib, activation)
     return topk_sum(contrib, topk_ids, E)
+
+
+def _adapted_layer(x, topk_weights, topk_ids, w13, w13_scale, w2, w2_scale, expert_map, num_experts, activation,
+                   adapters, adapter_ids):
+    """``fused_moe`` with low-rank adapters: the separate calls, the adapters' launches between them."""
+    if topk_ids.dim() != 2 or topk_ids.shape != topk_weights.shape:
+        raise ValueError(f"topk_ids {tuple(topk_ids.shape)} and topk_weights {tuple(topk_weights.shape)} must both be "
+                         "(T, topk)")
+    S, I = _slab(x.shape[1], w13, w13_scale, w2, w2_scale)
+    slots = min(S, MAX_SLOTS)
+    if expert_map is None:
+        expert_map = torch.arange(num_experts, dtype=torch.int32, device=x.device)
+    adapted = lora.adapt(x, adapters, adapter_ids, topk_ids, I, num_experts)
+    xq, xs, r = quant_route(x, topk_ids, expert_map, slots)
+    r.experts = num_experts
+    # Pairs without a slot are written by nothing and add nothing.
+    contrib = torch.zeros((topk_ids.numel(), x.shape[1]), dtype=torch.bfloat16, device=x.device)
+    run_experts(xq, xs, topk_weights, w13, w13_scale, w2, w2_scale, r, contrib, activation, adapted)
+    return topk_sum(contrib, topk_ids, num_experts)
 
 
 def _layer(x, topk_weights, topk_ids, w13, w13_scale, w2, w2_scale, expert_map, num_experts, activation):

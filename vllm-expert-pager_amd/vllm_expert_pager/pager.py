@@ -23,7 +23,7 @@ from typing import Callable
 
 import torch
 
-from vllm_expert_pager import moe, trace
+from vllm_expert_pager import lora, moe, trace
 from vllm_expert_pager.acquire import AcquirePair
 from vllm_expert_pager.codec import decode_rows_from_ram
 from vllm_expert_pager.gather import as_rows, fetch_publish_rows, fetch_wait_rows, gather_rows
@@ -213,7 +213,8 @@ class PagedExperts:
     # ---- forward ----
 
     def forward(self, x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor,
-                shared: Callable[[], object] | None = None) -> torch.Tensor:
+                shared: Callable[[], object] | None = None, adapters: lora.ExpertAdapters | None = None,
+                adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
         """The routed-expert output ``(T, H)`` bf16 of this layer (experts.py:380-453).
 
         ``shared``, if given, runs the layer's shared experts. It is called
@@ -221,9 +222,19 @@ class PagedExperts:
         decode path before the expert FFN, on the overflow path before
         chunk 0's (experts.py:452, 569-573). Its result is not part of the
         returned routed sum.
+
+        ``adapters`` add the requests' low-rank adapters beside the layer's
+        experts, token t's being ``adapter_ids[t]`` (-1: none). They are
+        addressed by expert id and stay in HBM, so they take no part in the
+        paging; the reference has no counterpart.
         """
         if not self.ready:
             raise RuntimeError(f"layer {self.layer}: setup() has not run")
+        if (adapters is None) != (adapter_ids is None):
+            raise ValueError("adapters and adapter_ids go together")
+        adapted = None
+        if adapters is not None:
+            adapted = lora.adapt(x, adapters, adapter_ids, topk_ids, self.pager.intermediate, self.pager.num_experts)
         store = self.store
         if store.path is not None and store.synced is None:
             self.pager.flush()
@@ -232,7 +243,7 @@ class PagedExperts:
         # The path is chosen from the shape alone, so capture and replay of a
         # graph take the same path.
         if topk_ids.numel() > self.table.num_slots:
-            return self._forward_working(x, topk_weights, topk_ids, shared)
+            return self._forward_working(x, topk_weights, topk_ids, shared, adapted)
 
         layer, E = self.layer, self.pager.num_experts
         with trace.range(f"expert_pager L{layer} acquire"):
@@ -286,7 +297,7 @@ class PagedExperts:
         if shared is not None:
             shared()
         with trace.range(f"expert_pager L{layer} experts"):
-            if moe.decode_pays(x, topk_ids, self.pager.intermediate):
+            if adapted is None and moe.decode_pays(x, topk_ids, self.pager.intermediate):
                 slab = self.cache_slab
                 out = moe.decode_experts(x, topk_weights, topk_ids, self.expert_map, E, slab[PARAMS[0]],
                                          slab[SCALES[0]], slab[PARAMS[1]], slab[SCALES[1]], self.table.num_slots,
@@ -295,12 +306,14 @@ class PagedExperts:
                 return out
             xq, xs, routing = moe.quant_route(x, topk_ids, self.expert_map, self.table.num_slots)
             contrib = self._contrib(topk_weights, x)
-            self._run(self.cache_slab, xq, xs, topk_weights, topk_ids, contrib, routing)
+            # Every needed expert has a slot here, so the adapters need no map of the chunk.
+            self._run(self.cache_slab, xq, xs, topk_weights, topk_ids, contrib, routing, adapted)
         self._log()
         return moe.topk_sum(contrib, topk_ids, E)
 
     def _forward_working(self, x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor,
-                         shared: Callable[[], object] | None = None) -> torch.Tensor:
+                         shared: Callable[[], object] | None = None,
+                         adapted: lora.AdaptedBatch | None = None) -> torch.Tensor:
         """Prefill (K > S): the experts go through the W-row working slab in chunks (experts.py:455-577).
 
         The VRAM table is not updated; VRAM hits are copied raw from the cache
@@ -362,7 +375,7 @@ class PagedExperts:
                 self.expert_map.copy_(maps[k])
                 if k == 0 and shared is not None:
                     shared()
-                self._run(p.working_slab, xq, xs, topk_weights, topk_ids, contrib)
+                self._run(p.working_slab, xq, xs, topk_weights, topk_ids, contrib, None, adapted, self.expert_map)
         self._log()
         return moe.topk_sum(contrib, topk_ids, E)
 
@@ -376,12 +389,13 @@ class PagedExperts:
         return torch.empty((T * topk, x.shape[1]), dtype=torch.bfloat16, device=x.device)
 
     def _run(self, slab: dict[str, torch.Tensor], xq: torch.Tensor, xs: torch.Tensor, topk_weights: torch.Tensor,
-             topk_ids: torch.Tensor, contrib: torch.Tensor, routing: moe.Routing | None = None) -> None:
+             topk_ids: torch.Tensor, contrib: torch.Tensor, routing: moe.Routing | None = None,
+             adapted: lora.AdaptedBatch | None = None, expert_map: torch.Tensor | None = None) -> None:
         """Run the experts that ``expert_map`` places in ``slab`` (experts.py:579-604)."""
         S = slab[PARAMS[0]].shape[0]
         r = routing if routing is not None else moe.route(topk_ids, self.expert_map, S)
         moe.run_experts(xq, xs, topk_weights, slab[PARAMS[0]], slab[SCALES[0]], slab[PARAMS[1]], slab[SCALES[1]],
-                        r, contrib, self.activation)
+                        r, contrib, self.activation, adapted, expert_map)
 
     # ---- counters ----
 
