@@ -21,8 +21,12 @@
 // row's sum), loss = sum f_e P_e, averaged over the sequences that have
 // tokens.
 //
-// A row is one wave's: lane l holds the VPL experts l * VPL .. l * VPL + VPL -
-// 1, so the first lane that holds the largest key also holds the lowest index.
+// Two forms. Up to 512 experts and 16 choices without bias and groups, a row is
+// 16 lanes' (four rows a wave): lane l holds the VPL experts l * VPL .. l * VPL
+// + VPL - 1, and the choice is a merge of sorted lists, with no step that waits
+// on the one before it for long. Otherwise a row is a wave's, and the choice a
+// round per expert: the largest key of all lanes, its first holder, and that
+// key taken out.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
@@ -104,10 +108,11 @@ __device__ __forceinline__ double key_value(uint64_t k) {
 }
 
 // ---- a row's logits: masked ones as -inf ----
-template <typename T, int VPL>
-__device__ __forceinline__ void load_row(const T* __restrict__ row, int E, bool vec, float (&z)[VPL]) {
+// LANES lanes hold a row, VPL consecutive experts each.
+template <typename T, int VPL, int LANES>
+__device__ __forceinline__ void load_part(const T* __restrict__ row, int E, bool vec, float (&z)[VPL]) {
   constexpr int kBytes = VPL * static_cast<int>(sizeof(T));
-  const int i0 = static_cast<int>(threadIdx.x & 63) * VPL;
+  const int i0 = static_cast<int>(threadIdx.x & (LANES - 1)) * VPL;
   if (kBytes >= 4 && vec && i0 + VPL <= E) {
     T v[VPL];
     if constexpr (kBytes % 16 == 0) {
@@ -327,7 +332,7 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(Rows r, Pick pk, float
   if (!r.mask || r.mask[t]) {
     const T* row = static_cast<const T*>(r.logits) + t * r.stride;
     float z[VPL];
-    load_row<T, VPL>(row, r.E, r.vec, z);
+    load_part<T, VPL, 64>(row, r.E, r.vec, z);
     choose_row<T, VPL, WIDE>(row, z, r.E, pk, s_raw + static_cast<size_t>(wave) * r.E * (WIDE ? 8 : 4), id, w);
   }
   if (lane < pk.topk) {
@@ -336,14 +341,45 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(Rows r, Pick pk, float
   }
 }
 
-// Partial sums of one workgroup's rows of a sequence: [seq][part][E].
+// What the workgroups hand to the join.
 struct Partial {
-  float* p;        // sums of the probabilities
-  int32_t* c;      // counts
+  uint2* pc;       // [seq][part][E]: sum of the probabilities (fp32 bits), count
   int32_t* n;      // [seq][part] valid tokens
   int parts;
-  double* loss;    // [seq]
+  double* loss;    // [seq][expert block]: the block's part of the sequence's loss (-1: no tokens)
+  int32_t* done;   // join workgroups that are done
 };
+
+// A workgroup's sums ([waves][pitch] in LDS), counts and valid tokens.
+__device__ __forceinline__ void store_partial(const Partial& out, int s, int j, int E, const int32_t* s_count,
+                                              const float* s_sum, int pitch, const int* s_valid) {
+  const int tid = threadIdx.x;
+  const int64_t part = static_cast<int64_t>(s) * out.parts + j;
+  for (int i = tid; i < E; i += kThreads) {
+    float a = s_sum[i];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) a += s_sum[w * pitch + i];
+    out.pc[part * E + i] = make_uint2(__float_as_uint(a), static_cast<uint32_t>(s_count[i]));
+  }
+  if (tid == 0) {
+    int n = 0;
+    for (int w = 0; w < kWaves; ++w) n += s_valid[w];
+    out.n[part] = n;
+  }
+}
+
+// The rows before and behind the sequences: no choice. Part j of `parts`.
+__device__ __forceinline__ void mark_padding(const Rows& r, int topk, float* weights, int32_t* ids, int j, int parts) {
+  int64_t first = r.offsets[0], last = r.offsets[r.num_seqs];
+  first = first < 0 ? 0 : (first < r.T ? first : r.T);
+  last = last < first ? first : (last < r.T ? last : r.T);
+  const int64_t n = (first + r.T - last) * topk;
+  for (int64_t i = static_cast<int64_t>(j) * kThreads + threadIdx.x; i < n; i += static_cast<int64_t>(parts) * kThreads) {
+    const int64_t at = i < first * topk ? i : i + (last - first) * topk;
+    ids[at] = -1;
+    weights[at] = 0.0f;
+  }
+}
 
 // Workgroup (part j, sequence s): rows lo + 4 j + wave, + 4 parts, ... of the
 // sequence; the sequence num_seqs stands for the rows outside all of them.
@@ -360,18 +396,9 @@ __global__ void __launch_bounds__(kThreads) balance_kernel(Rows r, Pick pk, cons
   __shared__ int s_valid[kWaves];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int s = blockIdx.y, j = blockIdx.x, E = r.E;
-  if (s == r.num_seqs) {  // padding before and behind the sequences
-    if constexpr (CHOOSE) {
-      int64_t first = r.offsets[0], last = r.offsets[r.num_seqs];
-      first = first < 0 ? 0 : (first < r.T ? first : r.T);
-      last = last < first ? first : (last < r.T ? last : r.T);
-      const int64_t n = (first + r.T - last) * pk.topk;
-      for (int64_t i = static_cast<int64_t>(j) * kThreads + tid; i < n; i += static_cast<int64_t>(out.parts) * kThreads) {
-        const int64_t at = i < first * pk.topk ? i : i + (last - first) * pk.topk;
-        ids[at] = -1;
-        weights[at] = 0.0f;
-      }
-    }
+  if (s == 0 && j == 0 && tid == 0) *out.done = 0;
+  if (s == r.num_seqs) {
+    if constexpr (CHOOSE) mark_padding(r, pk.topk, weights, ids, j, out.parts);
     return;
   }
   for (int i = tid; i < E; i += kThreads) s_count[i] = 0;
@@ -388,7 +415,7 @@ __global__ void __launch_bounds__(kThreads) balance_kernel(Rows r, Pick pk, cons
     if (on) {
       const T* row = static_cast<const T*>(r.logits) + t * r.stride;
       float z[VPL], term[VPL];
-      load_row<T, VPL>(row, E, r.vec, z);
+      load_part<T, VPL, 64>(row, E, r.vec, z);
       if constexpr (CHOOSE) {
         int mine;
         float w;
@@ -420,19 +447,7 @@ __global__ void __launch_bounds__(kThreads) balance_kernel(Rows r, Pick pk, cons
     if (lane * VPL + i < E) s_sum[wave * E + lane * VPL + i] = sum[i];
   if (lane == 0) s_valid[wave] = valid;
   __syncthreads();
-  const int64_t part = static_cast<int64_t>(s) * out.parts + j;
-  for (int i = tid; i < E; i += kThreads) {
-    float a = s_sum[i];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) a += s_sum[w * E + i];
-    out.p[part * E + i] = a;
-    out.c[part * E + i] = s_count[i];
-  }
-  if (tid == 0) {
-    int n = 0;
-    for (int w = 0; w < kWaves; ++w) n += s_valid[w];
-    out.n[part] = n;
-  }
+  store_partial(out, s, j, E, s_count, s_sum, E, s_valid);
 }
 
 // Sum of v over the workgroup, in every thread of wave 0 at least.
@@ -446,49 +461,442 @@ __device__ __forceinline__ double block_sum(double v, double* s_tmp) {
   return all;
 }
 
-// One sequence: its counts, valid tokens and loss from the partial sums, in 64 bits.
-__global__ void __launch_bounds__(kThreads) balance_join_kernel(Partial in, int E, int topk,
+constexpr int kJoinExperts = 16;  // experts of a join workgroup (128 bytes of a part's row)
+
+// Workgroup (expert block, sequence): the block's counts and its part of the
+// loss, from the partial sums, in 64 bits. The workgroup that is done last
+// adds the parts up, in the order of sequences and blocks whoever it is.
+__global__ void __launch_bounds__(kThreads) balance_join_kernel(Partial in, int E, int topk, int num_seqs,
                                                                 int32_t* __restrict__ counts,
-                                                                int32_t* __restrict__ tokens) {
+                                                                int32_t* __restrict__ tokens,
+                                                                float* __restrict__ loss) {
+  constexpr int kAcross = kThreads / kJoinExperts;  // parts summed side by side
   __shared__ double s_tmp[kWaves];
-  const int s = blockIdx.x, tid = threadIdx.x;
+  __shared__ double s_p[kAcross][kJoinExperts];
+  __shared__ int s_c[kAcross][kJoinExperts];
+  __shared__ int s_last;
+  const int s = blockIdx.y, tid = threadIdx.x;
+  const int x = tid % kJoinExperts, y = tid / kJoinExperts, e = blockIdx.x * kJoinExperts + x;
   const int64_t base = static_cast<int64_t>(s) * in.parts;
-  double n = 0.0;
+  double n = 0.0, p = 0.0;
+  int c = 0;
+  if (e < E) {
+#pragma unroll 8
+    for (int j = y; j < in.parts; j += kAcross) {
+      const uint2 v = in.pc[(base + j) * E + e];
+      p += __uint_as_float(v.x);
+      c += static_cast<int>(v.y);
+    }
+  }
   for (int j = tid; j < in.parts; j += kThreads) n += in.n[base + j];
+  s_p[y][x] = p;
+  s_c[y][x] = c;
   n = block_sum(n, s_tmp);
-  double loss = 0.0;
-  for (int e = tid; e < E; e += kThreads) {
-    double p = 0.0;
-    int32_t c = 0;
-    for (int j = 0; j < in.parts; ++j) {
-      p += in.p[(base + j) * E + e];
-      c += in.c[(base + j) * E + e];
+  double part = 0.0;
+  if (tid < kJoinExperts && e < E) {
+    for (int i = 1; i < kAcross; ++i) {
+      p += s_p[i][x];
+      c += s_c[i][x];
     }
     counts[static_cast<int64_t>(s) * E + e] = c;
-    loss += p * c;
+    part = p * c;
   }
-  loss = block_sum(loss, s_tmp);
+  part = block_sum(part, s_tmp);
   if (tid == 0) {
-    tokens[s] = static_cast<int32_t>(n);
-    in.loss[s] = n > 0.0 ? loss * E / (n * n * topk) : 0.0;
+    if (blockIdx.x == 0) tokens[s] = static_cast<int32_t>(n);
+    in.loss[static_cast<int64_t>(s) * gridDim.x + blockIdx.x] = n > 0.0 ? part * E / (n * n * topk) : -1.0;
+    const int total = static_cast<int>(gridDim.x * gridDim.y);
+    s_last = __hip_atomic_fetch_add(in.done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == total - 1;
   }
-}
-
-// The mean over the sequences with tokens; tokens[num_seqs] = their number.
-__global__ void __launch_bounds__(kThreads) balance_mean_kernel(Partial in, int num_seqs, int32_t* __restrict__ tokens,
-                                                                float* __restrict__ loss) {
-  __shared__ double s_tmp[kWaves];
+  __syncthreads();
+  if (!s_last) return;
   double a = 0.0, used = 0.0;
-  for (int s = threadIdx.x; s < num_seqs; s += kThreads) {
-    a += in.loss[s];
-    used += tokens[s] > 0 ? 1.0 : 0.0;
+  const int64_t all = static_cast<int64_t>(num_seqs) * gridDim.x;
+  for (int64_t i = tid; i < all; i += kThreads) {
+    const double v = __hip_atomic_load(in.loss + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (v < 0.0) continue;
+    a += v;
+    used += i % gridDim.x == 0 ? 1.0 : 0.0;
   }
   a = block_sum(a, s_tmp);
   used = block_sum(used, s_tmp);
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
     tokens[num_seqs] = static_cast<int32_t>(used);
     *loss = static_cast<float>(used > 0.0 ? a / used : 0.0);
   }
+}
+
+// ---- rows of 16 lanes ----
+
+constexpr int kRowLanes = 16;
+constexpr int kRowsPerWave = 64 / kRowLanes;
+constexpr int kBlockRows = kWaves * kRowsPerWave;
+constexpr int kNarrowExperts = 512;  // experts of a row of 16 lanes, at most (32 a lane)
+constexpr int kNarrowTopk = 16;      // chosen experts, at most (a lane each)
+
+// v of the lane that the DPP control names, within the row of 16 lanes.
+template <int CTRL>
+__device__ __forceinline__ uint32_t row_move(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), CTRL, 0xF, 0xF, false));
+}
+template <int CTRL>
+__device__ __forceinline__ float row_move(float v) {
+  return __uint_as_float(row_move<CTRL>(__float_as_uint(v)));
+}
+template <int CTRL>
+__device__ __forceinline__ double row_move(double v) {
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v));
+  const uint64_t lo = row_move<CTRL>(static_cast<uint32_t>(b)), hi = row_move<CTRL>(static_cast<uint32_t>(b >> 32));
+  return __longlong_as_double(static_cast<long long>(hi << 32 | lo));
+}
+// Lane distances 1 and 2, then the mirrors of 8 and of 16 lanes: after each
+// step all lanes of 2, 4, 8 and 16 hold the same result.
+constexpr int kSwap1 = 0xB1, kSwap2 = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140;
+
+__device__ __forceinline__ float row_sum(float v) {
+  v += row_move<kSwap1>(v);
+  v += row_move<kSwap2>(v);
+  v += row_move<kMirror8>(v);
+  return v + row_move<kMirror16>(v);
+}
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, row_move<kSwap1>(v));
+  v = fmaxf(v, row_move<kSwap2>(v));
+  v = fmaxf(v, row_move<kMirror8>(v));
+  return fmaxf(v, row_move<kMirror16>(v));
+}
+
+// e^x for x <= 0 (NaN and anything below -200: 0). x = (n + f) ln 2 with |f|
+// at most a half, f exact to 2^-26 through a second term of 1 / ln 2, and 2^f
+// by the instruction, good to one step; n goes into the exponent. 7
+// instructions, without the library's branches for other x.
+__device__ __forceinline__ float exp_below(float x) {
+  constexpr float kHi = 1.4426950408889634f;
+  constexpr float kLo = static_cast<float>(1.4426950408889634 - static_cast<double>(kHi));
+  x = fmaxf(x, -200.0f);
+  const float n = rintf(x * kHi);
+  const float f = fmaf(x, kLo, fmaf(x, kHi, -n));
+  return ldexpf(__builtin_amdgcn_exp2f(f), static_cast<int>(n));
+}
+
+// 1 / x for x >= 1: the instruction's one step of error, taken out by one
+// Newton step (an infinite x gives 0).
+__device__ __forceinline__ float reciprocal(float x) {
+  const float r = __builtin_amdgcn_rcpf(x);
+  return x < INFINITY ? fmaf(fmaf(-x, r, 1.0f), r, r) : 0.0f;
+}
+
+// A choice key with the expert's index in its low bits (the complement, so
+// that of equal logits the lower index is larger): all keys differ, and one
+// maximum finds both. 16-bit logits, seen as fp32, leave 13 low bits free, so
+// their keys fit 32 bits; an fp32 logit's key and index go into the fraction
+// of a double in [1, 2), whose maximum is one instruction too. kNone: masked.
+template <typename T>
+struct Key {
+  using type = uint32_t;
+  static constexpr uint32_t kField = 0x1fff;
+  static __device__ __forceinline__ type none() { return 0; }
+  static __device__ __forceinline__ type pack(float z, int i) {
+    const uint32_t k = order_key(z);
+    return k ? (k & ~kField) | (kField - static_cast<uint32_t>(i)) : 0;
+  }
+  static __device__ __forceinline__ int index(type k) { return k ? static_cast<int>(kField - (k & kField)) : -1; }
+  static __device__ __forceinline__ float value(type k) {
+    const uint32_t b = k >> 31 ? (k & ~kField) ^ 0x80000000u : ~(k | kField);
+    return k ? __uint_as_float(b) : -INFINITY;
+  }
+};
+template <>
+struct Key<float> {
+  using type = double;
+  static constexpr uint32_t kField = 0x7ff;
+  static __device__ __forceinline__ type none() { return 1.0; }
+  static __device__ __forceinline__ type pack(float z, int i) {
+    const uint32_t k = order_key(z);
+    const uint64_t b = 0x3ff0000000000000ull | static_cast<uint64_t>(k) << 11 | (kField - static_cast<uint32_t>(i));
+    return k ? __longlong_as_double(static_cast<long long>(b)) : none();
+  }
+  static __device__ __forceinline__ uint64_t bits(type k) {
+    return static_cast<uint64_t>(__double_as_longlong(k)) & 0x000fffffffffffffull;
+  }
+  static __device__ __forceinline__ int index(type k) {
+    const uint64_t b = bits(k);
+    return b ? static_cast<int>(kField - (b & kField)) : -1;
+  }
+  static __device__ __forceinline__ float value(type k) {
+    const uint32_t o = static_cast<uint32_t>(bits(k) >> 11);
+    return o ? __uint_as_float(o >> 31 ? o ^ 0x80000000u : ~o) : -INFINITY;
+  }
+};
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t smaller(uint32_t a, uint32_t b) { return a > b ? b : a; }
+__device__ __forceinline__ double larger(double a, double b) { return __builtin_fmax(a, b); }
+__device__ __forceinline__ double smaller(double a, double b) { return __builtin_fmin(a, b); }
+
+// A list that rises and falls once, sorted (largest first).
+template <int N, typename K>
+__device__ __forceinline__ void sort_merged(K (&a)[N]) {
+#pragma unroll
+  for (int d = N / 2; d > 0; d >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((i & d) == 0) {
+        const K x = a[i], y = a[i + d];
+        a[i] = larger(x, y);
+        a[i + d] = smaller(x, y);
+      }
+}
+template <int N, typename K>
+__device__ __forceinline__ void sort_list(K (&a)[N]) {
+#pragma unroll
+  for (int k = 2; k <= N; k <<= 1)
+#pragma unroll
+    for (int d = k / 2; d > 0; d >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if ((i & d) == 0) {
+          const K x = a[i], y = a[i + d];
+          const bool falls = (i & k) == 0;
+          a[i] = falls ? larger(x, y) : smaller(x, y);
+          a[i + d] = falls ? smaller(x, y) : larger(x, y);
+        }
+}
+// The N largest of two sorted lists, sorted.
+template <int N, typename K>
+__device__ __forceinline__ void merge_lists(K (&a)[N], const K (&b)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) a[i] = larger(a[i], b[N - 1 - i]);
+  sort_merged<N>(a);
+}
+template <int CTRL, int N, typename K>
+__device__ __forceinline__ void merge_lanes(K (&a)[N]) {
+  K b[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) b[i] = row_move<CTRL>(a[i]);
+  merge_lists<N>(a, b);
+}
+
+// The row's N largest keys, sorted, in every lane of the row.
+template <typename T, int VPL, int N>
+__device__ __forceinline__ void row_best(const float (&z)[VPL], typename Key<T>::type (&best)[N]) {
+  using K = typename Key<T>::type;
+  const int i0 = static_cast<int>(threadIdx.x & (kRowLanes - 1)) * VPL;
+#pragma unroll
+  for (int at = 0; at < VPL; at += N) {
+    K part[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[i] = at + i < VPL ? Key<T>::pack(z[at + i < VPL ? at + i : 0], i0 + at + i) : Key<T>::none();
+    sort_list<N>(part);
+    if (at == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) best[i] = part[i];
+    } else {
+      merge_lists<N>(best, part);
+    }
+  }
+  merge_lanes<kSwap1, N>(best);
+  merge_lanes<kSwap2, N>(best);
+  merge_lanes<kMirror8, N>(best);
+  merge_lanes<kMirror16, N>(best);
+}
+
+// A row's terms t_i (see row_terms) and their sum, by its 16 lanes.
+template <int VPL, bool SIGMOID>
+__device__ __forceinline__ float narrow_terms(const float (&z)[VPL], float (&t)[VPL]) {
+  float m = z[0];
+#pragma unroll
+  for (int i = 1; i < VPL; ++i) m = fmaxf(m, z[i]);
+  m = row_max(m);
+  if constexpr (SIGMOID) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const float e = exp_below(-fabsf(z[i]));
+      t[i] = (z[i] > 0.0f ? 1.0f : e) * reciprocal(1.0f + e);
+    }
+    if (__any(m < 0.0f)) {  // all logits of a row below 0: by the largest
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (m < 0.0f) t[i] = z[i] > -INFINITY ? exp_below(z[i] - m) * reciprocal(1.0f + exp_below(z[i])) : 0.0f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) t[i] = exp_below(z[i] - m);
+    if (__any(m == INFINITY)) {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (m == INFINITY) t[i] = z[i] == m ? 1.0f : 0.0f;
+    }
+  }
+  float s[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) s[i] = t[i];
+#pragma unroll
+  for (int d = VPL / 2; d > 0; d >>= 1)
+#pragma unroll
+    for (int i = 0; i < d; ++i) s[i] += s[i + d];
+  return row_sum(s[0]);
+}
+
+// The weight of the row's k-th choice in its lane k, from the lane's own
+// chosen logit (id -1: none), the row's largest logit and the sum of its terms
+// (softmax over all experts only).
+template <bool SIGMOID>
+__device__ __forceinline__ float choice_weight(const Pick& pk, int id, float zc, float top, float all) {
+  if constexpr (SIGMOID) {
+    // In 64 bits; renormalised by the largest where all logits are below 0.
+    const double shift = pk.renorm ? fminf(top, 0.0f) : 0.0, zd = zc;
+    const double s = id < 0 ? 0.0 : zc > 0.0f ? 1.0 / (1.0 + exp(-zd)) : exp(zd - shift) / (1.0 + exp(zd));
+    double sum = 1.0;
+    if (pk.renorm) {
+      sum = s;
+      sum += row_move<kSwap1>(sum);
+      sum += row_move<kSwap2>(sum);
+      sum += row_move<kMirror8>(sum);
+      sum += row_move<kMirror16>(sum);
+    }
+    return id < 0 ? 0.0f : static_cast<float>(s / sum * static_cast<double>(pk.scale));
+  } else {
+    const float e = id < 0 ? 0.0f : expf(below(zc, top));
+    if (pk.renorm) all = row_sum(e);
+    return id < 0 ? 0.0f : e / all * pk.scale;
+  }
+}
+
+// The choice of a row from its N best: lane k's id and logit.
+template <typename T, int N>
+__device__ __forceinline__ void own_choice(const typename Key<T>::type (&best)[N], int topk, int& id, float& zc) {
+  const int l = threadIdx.x & (kRowLanes - 1);
+  typename Key<T>::type mine = Key<T>::none();
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i == l && i < topk) mine = best[i];
+  id = Key<T>::index(mine);
+  zc = Key<T>::value(mine);
+}
+
+template <typename T, int VPL, bool SIGMOID, int N>
+__global__ void __launch_bounds__(kThreads) choose_narrow_kernel(Rows r, Pick pk, float* __restrict__ weights,
+                                                                 int32_t* __restrict__ ids) {
+  const int l = threadIdx.x & (kRowLanes - 1);
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kBlockRows + (threadIdx.x >> 4);
+  const int64_t tc = t < r.T ? t : r.T - 1;
+  const bool on = t < r.T && (!r.mask || r.mask[tc]);
+  float z[VPL];
+  load_part<T, VPL, kRowLanes>(static_cast<const T*>(r.logits) + tc * r.stride, r.E, r.vec, z);
+  typename Key<T>::type best[N];
+  row_best<T, VPL, N>(z, best);
+  int id;
+  float zc, all = 1.0f;
+  own_choice<T, N>(best, pk.topk, id, zc);
+  if constexpr (!SIGMOID) {
+    if (!pk.renorm) {
+      float term[VPL];
+      all = narrow_terms<VPL, false>(z, term);
+    }
+  }
+  const float w = choice_weight<SIGMOID>(pk, id, zc, Key<T>::value(best[0]), all);
+  if (l < pk.topk && t < r.T) {
+    ids[t * pk.topk + l] = on ? id : -1;
+    weights[t * pk.topk + l] = on ? w : 0.0f;
+  }
+}
+
+// balance_kernel with rows of 16 lanes: a workgroup takes kBlockRows rows of
+// its sequence at a time, the next ones requested before the present ones are
+// worked on. N 0: the choice is given.
+template <typename T, int VPL, bool SIGMOID, int N>
+__global__ void __launch_bounds__(kThreads) balance_narrow_kernel(Rows r, Pick pk, const void* __restrict__ given,
+                                                                  int eb, float* __restrict__ weights,
+                                                                  int32_t* __restrict__ ids, Partial out) {
+  constexpr bool CHOOSE = N > 0;
+  __shared__ int32_t s_count[kRowLanes * VPL];
+  __shared__ float s_sum[kWaves][kRowLanes * VPL];
+  __shared__ int s_valid[kWaves];
+  const int tid = threadIdx.x, wave = tid >> 6, l = tid & (kRowLanes - 1);
+  const int s = blockIdx.y, j = blockIdx.x, E = r.E;
+  if (s == 0 && j == 0 && tid == 0) *out.done = 0;
+  if (s == r.num_seqs) {
+    if constexpr (CHOOSE) mark_padding(r, pk.topk, weights, ids, j, out.parts);
+    return;
+  }
+  for (int i = tid; i < E; i += kThreads) s_count[i] = 0;
+  __syncthreads();
+  int64_t lo, hi;
+  seq_range(r, s, lo, hi);
+  const int64_t step = static_cast<int64_t>(out.parts) * kBlockRows;
+  const T* const base = static_cast<const T*>(r.logits);
+  float sum[VPL], next[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) sum[i] = 0.0f;
+  int valid = 0;
+  const int64_t t0 = lo + static_cast<int64_t>(j) * kBlockRows;
+  auto clamped = [&](int64_t t) { return t < hi ? t : hi - 1; };
+  if (t0 < hi) load_part<T, VPL, kRowLanes>(base + clamped(t0 + (tid >> 4)) * r.stride, E, r.vec, next);
+  for (int64_t tb = t0; tb < hi; tb += step) {
+    const int64_t t = tb + (tid >> 4);
+    float z[VPL], term[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) z[i] = next[i];
+    if (tb + step < hi) load_part<T, VPL, kRowLanes>(base + clamped(t + step) * r.stride, E, r.vec, next);
+    const bool on = t < hi && (!r.mask || r.mask[t]);
+    int64_t id = -1;
+    if constexpr (!CHOOSE) {
+      if (l < pk.topk && on) id = load_id(given, eb, t * pk.topk + l);
+    }
+    const float all = narrow_terms<VPL, SIGMOID>(z, term);
+    if constexpr (CHOOSE) {
+      typename Key<T>::type best[N];
+      row_best<T, VPL, N>(z, best);
+      int own;
+      float zc;
+      own_choice<T, N>(best, pk.topk, own, zc);
+      const float w = choice_weight<SIGMOID>(pk, own, zc, Key<T>::value(best[0]), all);
+      if (l < pk.topk && t < hi) {
+        ids[t * pk.topk + l] = on ? own : -1;
+        weights[t * pk.topk + l] = on ? w : 0.0f;
+      }
+      id = on ? own : -1;
+    }
+    if (id >= 0 && id < E) atomicAdd(&s_count[id], 1);
+    const float inv = on && all > 0.0f ? 1.0f / all : 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) sum[i] = fmaf(term[i], inv, sum[i]);
+    valid += on;
+  }
+  // The wave's four rows of lanes, then the waves.
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum[i]), __float_as_uint(sum[i]), false, false);
+    const float v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    sum[i] = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+  }
+  valid += __shfl_xor(valid, 16, 64);
+  valid += __shfl_xor(valid, 32, 64);
+  if ((tid & 63) < kRowLanes) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) s_sum[wave][l * VPL + i] = sum[i];
+  }
+  if ((tid & 63) == 0) s_valid[wave] = valid;
+  __syncthreads();
+  store_partial(out, s, j, E, s_count, &s_sum[0][0], kRowLanes * VPL, s_valid);
+}
+
+// The sequence of row t (the last that starts at or before it), and whether
+// the row lies in it.
+__device__ __forceinline__ bool find_seq(const Rows& r, int64_t t, int& s) {
+  s = 0;
+  if (!r.offsets) return true;
+  int a = 0, z = r.num_seqs;
+  while (z - a > 1) {
+    const int m = (a + z) >> 1;
+    if (r.offsets[m] <= t)
+      a = m;
+    else
+      z = m;
+  }
+  s = a;
+  return r.offsets[s] <= t && t < r.offsets[s + 1];
 }
 
 struct Back {
@@ -511,27 +919,14 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(Rows r, Pick pk, Bac
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, E = r.E;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kWaves + wave;
   if (t >= r.T) return;
-  // The row's sequence: the last one that starts at or before it, and ends behind it.
-  int s = 0;
-  bool on = !r.mask || r.mask[t];
-  if (on && r.offsets) {
-    int a = 0, z = r.num_seqs;
-    while (z - a > 1) {
-      const int m = (a + z) >> 1;
-      if (r.offsets[m] <= t)
-        a = m;
-      else
-        z = m;
-    }
-    s = a;
-    on = r.offsets[s] <= t && t < r.offsets[s + 1];
-  }
+  int s;
+  const bool on = find_seq(r, t, s) && (!r.mask || r.mask[t]);
   float z[VPL], p[VPL], dz[VPL];
 #pragma unroll
   for (int i = 0; i < VPL; ++i) dz[i] = 0.0f;
   if (on) {
     const T* row = static_cast<const T*>(r.logits) + t * r.stride;
-    load_row<T, VPL>(row, E, r.vec, z);
+    load_part<T, VPL, 64>(row, E, r.vec, z);
     const float all = row_terms<VPL, SIGMOID>(z, p);
     const float inv = all > 0.0f ? 1.0f / all : 0.0f;
     float G[VPL];
@@ -613,6 +1008,138 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(Rows r, Pick pk, Bac
     if (lane * VPL + i < E) store_as(grad + t * E + lane * VPL + i, dz[i]);
 }
 
+template <typename T, int VPL>
+__device__ __forceinline__ void store_part(T* __restrict__ row, int E, bool vec, const float (&v)[VPL]) {
+  constexpr int kBytes = VPL * static_cast<int>(sizeof(T));
+  const int i0 = static_cast<int>(threadIdx.x & (kRowLanes - 1)) * VPL;
+  if (kBytes >= 4 && vec && i0 + VPL <= E) {
+    T o[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) store_as(&o[i], v[i]);
+    if constexpr (kBytes % 16 == 0) {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i)
+        reinterpret_cast<u32x4*>(row + i0)[i] = reinterpret_cast<const u32x4*>(o)[i];
+    } else if constexpr (kBytes == 8) {
+      *reinterpret_cast<uint2*>(row + i0) = *reinterpret_cast<const uint2*>(o);
+    } else if constexpr (kBytes == 4) {
+      *reinterpret_cast<uint32_t*>(row + i0) = *reinterpret_cast<const uint32_t*>(o);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (i0 + i < E) store_as(row + i0 + i, v[i]);
+  }
+}
+
+// backward_kernel with rows of 16 lanes. The chosen experts' own terms are
+// added by the lane that holds the choice, which writes that element again
+// behind the row's store, instead of a search for it among the row's lanes.
+template <typename T, int VPL, bool SIGMOID>
+__global__ void __launch_bounds__(kThreads) backward_narrow_kernel(Rows r, Pick pk, Back b, T* __restrict__ grad,
+                                                                   bool grad_vec) {
+  const int l = threadIdx.x & (kRowLanes - 1), E = r.E;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kBlockRows + (threadIdx.x >> 4);
+  const int64_t tc = t < r.T ? t : r.T - 1;
+  const T* row = static_cast<const T*>(r.logits) + tc * r.stride;
+  float z[VPL], p[VPL];
+  load_part<T, VPL, kRowLanes>(row, E, r.vec, z);
+  int s;
+  const bool on = find_seq(r, tc, s) && (!r.mask || r.mask[tc]);
+  int id = -1;
+  float g = 0.0f, zc = -INFINITY;
+  if (b.grad_weights && l < pk.topk) {
+    const int64_t e = load_id(b.ids, b.eb, tc * pk.topk + l);
+    id = e >= 0 && e < E ? static_cast<int>(e) : -1;
+    if (id >= 0) {
+      g = b.grad_weights[tc * pk.topk + l] * pk.scale;
+      zc = to_float(row[id]);
+      zc = zc > -INFINITY ? zc : -INFINITY;
+    }
+  }
+  float k = 0.0f;  // G_i = k counts_i
+  const int32_t* count = nullptr;
+  if (b.counts) {
+    const float n = static_cast<float>(b.tokens[s]);
+    k = n > 0.0f ? *b.grad_loss * static_cast<float>(E) /
+                       (n * n * static_cast<float>(pk.topk) * static_cast<float>(b.tokens[r.num_seqs]))
+                 : 0.0f;
+    count = b.counts + static_cast<int64_t>(s) * E;
+  }
+  const float all = narrow_terms<VPL, SIGMOID>(z, p);
+  const float inv = all > 0.0f ? 1.0f / all : 0.0f;
+  float G[VPL], dot = 0.0f;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    p[i] *= inv;
+    G[i] = 0.0f;
+  }
+  if (count) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (l * VPL + i < E) G[i] = k * static_cast<float>(count[l * VPL + i]);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) dot = fmaf(G[i], p[i], dot);
+  }
+  // The lane's own choice: its share of the weights, probability and slope.
+  float w = 0.0f, pc = 0.0f, slope = 1.0f, own = 0.0f;
+  const bool mine = id >= 0 && on;
+  if (b.grad_weights) {
+    const float top = row_max(zc);
+    const float ez = SIGMOID ? exp_below(-fabsf(zc)) : 0.0f;
+    float e = 0.0f;
+    if constexpr (SIGMOID) {
+      const float inv1 = reciprocal(1.0f + ez);
+      slope = (zc > 0.0f ? ez : 1.0f) * inv1;
+      e = (zc > 0.0f ? 1.0f : exp_below(zc - fminf(top, 0.0f))) * inv1;
+      own = (zc > 0.0f ? 1.0f : ez) * inv1;  // the score itself
+    } else {
+      e = exp_below(below(zc, top));
+    }
+    if (id < 0) e = 0.0f;
+    if (pk.renorm) {
+      const float sum = row_sum(e);
+      w = sum > 0.0f ? e / sum : 0.0f;
+    }
+    // p_c: the row's own p at the chosen expert, from the same logit.
+    float m = z[0];
+#pragma unroll
+    for (int i = 1; i < VPL; ++i) m = fmaxf(m, z[i]);
+    m = row_max(m);
+    if constexpr (SIGMOID)
+      pc = (m < 0.0f ? exp_below(zc - m) * reciprocal(1.0f + ez) : own) * inv;
+    else
+      pc = exp_below(below(zc, m)) * inv;
+    if (id < 0) pc = 0.0f;
+    if (!SIGMOID && !pk.renorm) dot = fmaf(g, pc, dot);
+  }
+  if (count || (!SIGMOID && !pk.renorm)) dot = row_sum(dot);
+  float dz[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    dz[i] = on ? p[i] * (G[i] - dot) : 0.0f;
+    if (SIGMOID && count) {  // 1 - s
+      const float e = exp_below(-fabsf(z[i]));
+      dz[i] *= (z[i] > 0.0f ? e : 1.0f) * reciprocal(1.0f + e);
+    }
+  }
+  if (t < r.T) store_part<T, VPL>(grad + t * E, E, grad_vec, dz);
+  if (b.grad_weights) {
+    const float gw = pk.renorm ? row_sum(g * w) : 0.0f;
+    float v = pc * ((count && id >= 0 ? k * static_cast<float>(count[id]) : 0.0f) - dot);
+    if (SIGMOID) v *= slope;
+    if (pk.renorm)
+      v += w * slope * (g - gw);
+    else if (SIGMOID)
+      v += g * own * slope;
+    else
+      v += pc * g;
+    // Behind the row's store, and kept there: the two go to the same address.
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    if (mine && t < r.T) store_as(grad + t * E + id, v);
+  }
+}
+
 // ---- host side ----
 
 struct Call {
@@ -654,14 +1181,17 @@ int check_pick(const char* what, int64_t E, int64_t topk, int scoring, int64_t g
 size_t elem_bytes(int dtype) { return dtype == XP_FLOAT32 ? 4 : 2; }
 
 // The experts a lane holds: the least power of two that covers E.
-int values_per_lane(int64_t E) {
+int values_per_lane(int64_t E, int lanes) {
   int v = 1;
-  while (64 * v < E) v *= 2;
+  while (lanes * v < E) v *= 2;
   return v;
 }
 
-Rows rows_of(const Call& c) {
-  const size_t eb = elem_bytes(c.dtype), chunk = std::min<size_t>(16, values_per_lane(c.E) * eb);
+// Whether rows are 16 lanes' (see the top).
+bool narrow_rows(int64_t E, int64_t topk) { return E <= kNarrowExperts && topk <= kNarrowTopk; }
+
+Rows rows_of(const Call& c, int lanes) {
+  const size_t eb = elem_bytes(c.dtype), chunk = std::min<size_t>(16, values_per_lane(c.E, lanes) * eb);
   Rows r{c.logits, c.T, c.stride, static_cast<int>(c.E), false, c.mask, c.offsets, static_cast<int>(c.num_seqs)};
   r.vec = reinterpret_cast<uintptr_t>(c.logits) % chunk == 0 && c.stride * eb % chunk == 0;
   return r;
@@ -691,25 +1221,27 @@ void dispatch(int dtype, int vpl, F&& f) {
   }
 }
 
-// Workgroups that share a sequence.
+// Workgroups that share a sequence: kBlockRows rows each at least, and no more
+// than about 512 in all (the join reads a row of E sums from each).
 int balance_parts(int64_t T, int64_t num_seqs) {
   const int64_t per = (T + num_seqs - 1) / num_seqs;
-  int64_t parts = (per + 4 * kWaves - 1) / (4 * kWaves);  // four rows a wave at least
-  parts = std::min<int64_t>(parts, std::max<int64_t>(1, 512 / num_seqs));
+  const int64_t parts = std::min<int64_t>((per + kBlockRows - 1) / kBlockRows, std::max<int64_t>(1, 512 / num_seqs));
   return static_cast<int>(std::max<int64_t>(parts, 1));
 }
 
 int64_t align256(int64_t n) { return (n + 255) & ~int64_t(255); }
 
+int64_t join_blocks(int64_t E) { return (E + kJoinExperts - 1) / kJoinExperts; }
+
 int64_t balance_layout(int64_t T, int64_t E, int64_t num_seqs, Partial* p, uint8_t* base) {
   const int64_t parts = balance_parts(T, num_seqs), n = parts * num_seqs;
-  const int64_t sz[4] = {align256(n * E * 4), align256(n * E * 4), align256(n * 4), align256(num_seqs * 8)};
+  const int64_t sz[4] = {align256(n * E * 8), align256(n * 4), align256(num_seqs * join_blocks(E) * 8), 256};
   if (p) {
     p->parts = static_cast<int>(parts);
-    p->p = reinterpret_cast<float*>(base);
-    p->c = reinterpret_cast<int32_t*>(base + sz[0]);
-    p->n = reinterpret_cast<int32_t*>(base + sz[0] + sz[1]);
-    p->loss = reinterpret_cast<double*>(base + sz[0] + sz[1] + sz[2]);
+    p->pc = reinterpret_cast<uint2*>(base);
+    p->n = reinterpret_cast<int32_t*>(base + sz[0]);
+    p->loss = reinterpret_cast<double*>(base + sz[0] + sz[1]);
+    p->done = reinterpret_cast<int32_t*>(base + sz[0] + sz[1] + sz[2]);
   }
   return sz[0] + sz[1] + sz[2] + sz[3];
 }
@@ -719,31 +1251,36 @@ int launch_balance(const Call& c, const Pick& pk, bool choose, const void* given
   const hipStream_t st = as_stream(stream);
   Partial part{};
   balance_layout(c.T, c.E, c.num_seqs, &part, static_cast<uint8_t*>(work));
+  const dim3 grid(static_cast<unsigned>(part.parts), static_cast<unsigned>(c.num_seqs + (choose && c.offsets ? 1 : 0)));
+  const bool narrow = narrow_rows(c.E, pk.topk) && !pk.bias && pk.groups == 1;
+  const int lanes = narrow ? kRowLanes : 64;
+  const Rows r = rows_of(c, lanes);
   const bool wide = choose && pk.bias;
   const size_t keys = choose && pk.groups > 1 ? static_cast<size_t>(kWaves) * c.E * (wide ? 8 : 4) : 0;
-  const size_t lds = ((c.E * 4 + 15) & ~size_t(15)) + std::max(keys, static_cast<size_t>(kWaves) * c.E * 4);
-  const dim3 grid(static_cast<unsigned>(part.parts), static_cast<unsigned>(c.num_seqs + (choose && c.offsets ? 1 : 0)));
-  const Rows r = rows_of(c);
-  dispatch(c.dtype, values_per_lane(c.E), [&](auto type, auto v) {
+  const size_t lds =
+      narrow ? 0 : ((c.E * 4 + 15) & ~size_t(15)) + std::max(keys, static_cast<size_t>(kWaves) * c.E * 4);
+  dispatch(c.dtype, values_per_lane(c.E, lanes), [&](auto type, auto v) {
     using T = decltype(type);
     constexpr int V = decltype(v)::value;
     auto go = [&](auto* kernel) {
       hipLaunchKernelGGL(kernel, grid, dim3(kThreads), lds, st, r, pk, given, eb, weights, ids, part);
     };
-    if (!choose)
-      pk.sigmoid ? go(balance_kernel<T, V, true, false, false>) : go(balance_kernel<T, V, false, false, false>);
-    else if (wide)
-      pk.sigmoid ? go(balance_kernel<T, V, true, true, true>) : go(balance_kernel<T, V, false, true, true>);
-    else
-      pk.sigmoid ? go(balance_kernel<T, V, true, true, false>) : go(balance_kernel<T, V, false, true, false>);
+    auto by_score = [&](auto sig) {
+      constexpr bool S = decltype(sig)::value != 0;
+      if (narrow)
+        !choose ? go(balance_narrow_kernel<T, V, S, 0>)
+                : pk.topk <= 8 ? go(balance_narrow_kernel<T, V, S, 8>) : go(balance_narrow_kernel<T, V, S, 16>);
+      else
+        !choose ? go(balance_kernel<T, V, S, false, false>)
+                : wide ? go(balance_kernel<T, V, S, true, true>) : go(balance_kernel<T, V, S, true, false>);
+    };
+    pk.sigmoid ? by_score(Int<1>{}) : by_score(Int<0>{});
   });
   if (int rc = check_launch("balance_kernel")) return rc;
-  hipLaunchKernelGGL(balance_join_kernel, dim3(static_cast<unsigned>(c.num_seqs)), dim3(kThreads), 0, st, part,
-                     static_cast<int>(c.E), pk.topk, counts, tokens);
-  if (int rc = check_launch("balance_join_kernel")) return rc;
-  hipLaunchKernelGGL(balance_mean_kernel, dim3(1), dim3(kThreads), 0, st, part, static_cast<int>(c.num_seqs), tokens,
-                     loss);
-  return check_launch("balance_mean_kernel");
+  hipLaunchKernelGGL(balance_join_kernel,
+                     dim3(static_cast<unsigned>(join_blocks(c.E)), static_cast<unsigned>(c.num_seqs)), dim3(kThreads), 0,
+                     st, part, static_cast<int>(c.E), pk.topk, static_cast<int>(c.num_seqs), counts, tokens, loss);
+  return check_launch("balance_join_kernel");
 }
 
 }  // namespace
@@ -764,14 +1301,23 @@ int xp_router_choose(const void* logits, int dtype, int64_t T, int64_t E, int64_
   XP_REQUIRE(weights && ids, "%s: null output", what);
   const Pick pk{static_cast<int>(topk), scoring == XP_SCORE_SIGMOID, renormalize != 0, static_cast<int>(groups),
                 static_cast<int>(topk_groups), static_cast<float>(scale), bias};
-  const Rows r = rows_of(c);
+  const bool narrow = narrow_rows(E, topk) && !bias && groups == 1;
+  const int lanes = narrow ? kRowLanes : 64, per_block = narrow ? kBlockRows : kWaves;
+  const Rows r = rows_of(c, lanes);
   const size_t lds = groups > 1 ? static_cast<size_t>(kWaves) * E * (bias ? 8 : 4) : 0;
-  const dim3 grid(static_cast<unsigned>((T + kWaves - 1) / kWaves));
-  dispatch(dtype, values_per_lane(E), [&](auto type, auto v) {
+  const dim3 grid(static_cast<unsigned>((T + per_block - 1) / per_block));
+  dispatch(dtype, values_per_lane(E, lanes), [&](auto type, auto v) {
     using L = decltype(type);
     constexpr int V = decltype(v)::value;
-    auto* kernel = bias ? choose_kernel<L, V, true> : choose_kernel<L, V, false>;
-    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), lds, as_stream(stream), r, pk, weights, ids);
+    auto go = [&](auto* kernel) {
+      hipLaunchKernelGGL(kernel, grid, dim3(kThreads), lds, as_stream(stream), r, pk, weights, ids);
+    };
+    if (!narrow)
+      bias ? go(choose_kernel<L, V, true>) : go(choose_kernel<L, V, false>);
+    else if (topk <= 8)
+      pk.sigmoid ? go(choose_narrow_kernel<L, V, true, 8>) : go(choose_narrow_kernel<L, V, false, 8>);
+    else
+      pk.sigmoid ? go(choose_narrow_kernel<L, V, true, 16>) : go(choose_narrow_kernel<L, V, false, 16>);
   });
   return check_launch("choose_kernel");
 }
@@ -840,13 +1386,22 @@ int xp_router_backward(const void* logits, int dtype, int64_t T, int64_t E, int6
   const Pick pk{static_cast<int>(topk), scoring == XP_SCORE_SIGMOID, renormalize != 0, 1, 1, static_cast<float>(scale),
                 nullptr};
   const Back b{topk_ids, topk_elem_bytes, grad_weights, counts, tokens, grad_loss};
-  const Rows r = rows_of(c);
-  const dim3 grid(static_cast<unsigned>((T + kWaves - 1) / kWaves));
-  dispatch(dtype, values_per_lane(E), [&](auto type, auto v) {
+  const bool narrow = narrow_rows(E, topk);
+  const int lanes = narrow ? kRowLanes : 64, per_block = narrow ? kBlockRows : kWaves;
+  const Rows r = rows_of(c, lanes);
+  const dim3 grid(static_cast<unsigned>((T + per_block - 1) / per_block));
+  dispatch(dtype, values_per_lane(E, lanes), [&](auto type, auto v) {
     using L = decltype(type);
     constexpr int V = decltype(v)::value;
-    auto* kernel = pk.sigmoid ? backward_kernel<L, V, true> : backward_kernel<L, V, false>;
-    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, as_stream(stream), r, pk, b, static_cast<L*>(grad));
+    const size_t chunk = std::min<size_t>(16, V * sizeof(L));
+    const bool vec = reinterpret_cast<uintptr_t>(grad) % chunk == 0 && E * sizeof(L) % chunk == 0;
+    if (narrow) {
+      auto* kernel = pk.sigmoid ? backward_narrow_kernel<L, V, true> : backward_narrow_kernel<L, V, false>;
+      hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, as_stream(stream), r, pk, b, static_cast<L*>(grad), vec);
+    } else {
+      auto* kernel = pk.sigmoid ? backward_kernel<L, V, true> : backward_kernel<L, V, false>;
+      hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, as_stream(stream), r, pk, b, static_cast<L*>(grad));
+    }
   });
   return check_launch("backward_kernel");
 }

@@ -200,6 +200,11 @@ def call(name: str, *args) -> None:
     check(getattr(lib(), name)(*args), name)
 
 
+# The current stream's handle without a Stream object around it.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def stream() -> int:
     """Raw hipStream_t of torch's current stream."""
     return torch.cuda.current_stream().cuda_stream
@@ -207,11 +212,14 @@ def stream() -> int:
 
 def call_on(t: torch.Tensor, name: str, *args) -> None:
     """``call`` with the current stream of t's device as the last argument, that device being the current one."""
-    if t.device.index == torch.cuda.current_device():
-        check(getattr(lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
-        return
-    with torch.cuda.device(t.device):
-        check(getattr(lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
+    device = t.get_device()
+    if device == torch.cuda.current_device():
+        rc = getattr(lib(), name)(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(lib(), name)(*args, _raw_stream(device))
+    if rc != XP_OK:
+        check(rc, name)
 
 
 def require_same_device(t: torch.Tensor, other: torch.Tensor, what: str) -> None:

@@ -112,16 +112,21 @@ def _backward(ctx, grad_weights, grad_loss):
     return grad
 
 
+def _choose(logits, topk, scoring, renormalize, bias, groups, topk_groups, scale, mask):
+    T, E = logits.shape
+    weights = logits.new_empty((T, topk), dtype=torch.float32)
+    ids = logits.new_empty((T, topk), dtype=torch.int32)
+    nat.call_on(
+        logits, "xp_router_choose", logits.data_ptr(), _DTYPES[logits.dtype], T, E, logits.stride(0), topk, scoring,
+        renormalize, nat.ptr(bias), groups, topk_groups, scale, nat.ptr(mask), weights.data_ptr(), ids.data_ptr(),
+    )
+    return weights, ids
+
+
 class _Choose(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, topk, scoring, renormalize, bias, groups, topk_groups, scale, mask):
-        T, E = logits.shape
-        weights = torch.empty((T, topk), dtype=torch.float32, device=logits.device)
-        ids = torch.empty((T, topk), dtype=torch.int32, device=logits.device)
-        nat.call_on(
-            logits, "xp_router_choose", logits.data_ptr(), _DTYPES[logits.dtype], T, E, logits.stride(0), topk, scoring,
-            renormalize, nat.ptr(bias), groups, topk_groups, scale, nat.ptr(mask), weights.data_ptr(), ids.data_ptr(),
-        )
+        weights, ids = _choose(logits, topk, scoring, renormalize, bias, groups, topk_groups, scale, mask)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(ids)
         ctx.save_for_backward(logits, ids, None, None, mask, None)
@@ -210,8 +215,10 @@ def choose_experts(
     code = _scoring(scoring)
     logits = _logits(logits)
     bias = _pick(logits, topk, bias, groups, topk_groups)
-    return _Choose.apply(logits, topk, code, bool(renormalize), bias, groups, topk_groups, float(scale),
-                         _mask(mask, logits))
+    args = (logits, topk, code, bool(renormalize), bias, groups, topk_groups, float(scale), _mask(mask, logits))
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Choose.apply(*args)
+    return _choose(*args)  # serving: no graph, and none of its cost (half of a one-token call's host time)
 
 
 def balance_loss(
