@@ -628,9 +628,11 @@ int xp_router_backward(const void* logits, int dtype, int64_t T, int64_t E,
  * No counterpart in the reference. The adapters of a projection of S slices
  * (2 for gate and up) of n columns from K inputs, for L adapters and E
  * experts, bf16 or fp16, R = the storage rank:
- *   a [L][E][S][R][Kp]   Kp = K rounded up to 32, zeros behind K and behind
- *                        an adapter's rank
- *   b [L][E][S][np][R]   np = n rounded up to 16, zeros likewise
+ *   a [L][E][S][R/16][Kp/32][4][16][8]   A by blocks of 16 ranks and 32
+ *                        inputs, rank 16 i + m, input 32 k + 8 q + c at [i][k]
+ *                        [q][m][c]; Kp = K rounded up to 32, zeros behind K
+ *                        and behind an adapter's rank
+ *   b [L][E][S][np][R]   np = n rounded up to 32, zeros likewise
  *   scales [L] (fp32), ranks [L] (int32, 0 .. R: what is read of a and b)
  * R is 16, 32, 64, 96 or 128; K and n are multiples of 8.
  */
@@ -660,7 +662,7 @@ int xp_lora_group(const void* adapter_ids, int adapter_elem_bytes,
  * base. Sums and the inner product in fp32 (the inner product enters the
  * second one as a sum of two values of the type). grouped != 0: the workspace
  * holds the listing of xp_lora_group for the same ids and sizes; else the call
- * makes it. Calls of at most 64 pairs group themselves and need no workspace. */
+ * makes it. Calls of at most 256 pairs group themselves and need no workspace. */
 int xp_lora_apply(const void* x, int dtype, int64_t x_stride, int per_pair,
                   int64_t T, int64_t topk, int64_t K, const void* a,
                   const void* b, const float* scales, const int32_t* ranks,

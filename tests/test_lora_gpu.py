@@ -110,21 +110,41 @@ def test_against_the_products(T, E, topk, K, n, slices, ranks, max_rank, L, dtyp
     assert torch.equal(got[none], base[none] if base is not None else torch.zeros_like(got[none]))
 
 
-def test_many_groups_and_pairs_of_one():
-    """A prefill over thousands of groups (some of them with many tiles), against a second call pair by pair."""
+@pytest.mark.parametrize("L, E, T, topk, dtype", [
+    (20, 256, 900, 4, torch.bfloat16),  # thousands of groups, some of many pairs
+    (2, 1, 6000, 1, torch.bfloat16),  # two groups of thousands
+    (3, 2, 20000, 1, torch.float16),  # tiles of 64 by the number of pairs
+    (1, 40, 130, 2, torch.bfloat16),  # just above what a workgroup groups itself
+    (1, 40, 128, 2, torch.bfloat16),  # and the most that it does
+])
+def test_any_order_and_any_split(L, E, T, topk, dtype):
+    """The order of the tokens changes no bit, nor does a second run; calls of a few tokens each agree within the
+    roundings: their sums run over other parts of K, two fp32 sums of K products apart at most, then one rounding."""
     lora = _lora()
     g = torch.Generator(device="cuda").manual_seed(0)
-    L, E, K, n, T, topk = 20, 256, 128, 64, 900, 4
-    stack, _ = _stack(L, E, K, n, [16, 3], 1, torch.bfloat16, 16, 1)
-    x = torch.randn((T, K), generator=g, device="cuda").to(torch.bfloat16)
+    K, n = 128, 64
+    stack, mats = _stack(L, E, K, n, [16, 3], 1, dtype, 16, 1)
+    x = torch.randn((T, K), generator=g, device="cuda").to(dtype)
     adapter = torch.randint(-1, L, (T,), generator=g, device="cuda")
-    adapter[::3] = 7
-    ids = torch.rand((T, E), generator=g, device="cuda").argsort(1)[:, :topk].to(torch.int32)
-    ids[::2, 0] = 11
-    whole = lora.low_rank(x, stack, adapter, ids)
-    parts = [lora.low_rank(x[t : t + 16], stack, adapter[t : t + 16], ids[t : t + 16]) for t in range(0, T, 16)]
-    assert torch.equal(whole, torch.cat(parts))  # a pair's result does not depend on the others
-    assert torch.equal(whole, lora.low_rank(x, stack, adapter, ids))
+    adapter[::3] = L // 2
+    ids = torch.rand((T, E), generator=g, device="cuda").argsort(1)[:, :topk].to(torch.int32).contiguous()
+    if E > 11:
+        ids[::2, 0] = 11
+    experts = ids if E > 1 else None
+    whole = lora.low_rank(x, stack, adapter, experts)
+    assert torch.equal(whole, lora.low_rank(x, stack, adapter, experts))
+    turn = torch.randperm(T, generator=g, device="cuda")
+    turned = lora.low_rank(x[turn], stack, adapter[turn], None if experts is None else experts[turn])
+    assert torch.equal(whole.view(T, topk, n)[turn], turned.view(T, topk, n))
+    step = 16
+    some = range(0, min(T, 2000), step)
+    parts = torch.cat([lora.low_rank(x[t : t + step], stack, adapter[t : t + step],
+                                     None if experts is None else experts[t : t + step]) for t in some])
+    a, b = whole[: parts.shape[0]].double(), parts.double()
+    # sum |B| (|A| |x|) is below 16 x 0.5 x 5 sigma ... taken from the largest matrices' rows
+    reach = max(float(m[2]) * m[1].double().abs().sum(-1).max().item() * m[0].double().abs().sum(-1).max().item()
+                for m in mats) * x.double().abs().max().item()
+    assert ((a - b).abs() <= 2 * HALF[dtype] * 1.01 * torch.maximum(a.abs(), b.abs()) + 4 * (K + 16) * U * reach).all()
 
 
 @pytest.mark.parametrize("T", [3, 200])

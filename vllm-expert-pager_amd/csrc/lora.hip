@@ -5,14 +5,18 @@
 //   scale B (A x)        A: [R][K], B: [n][R] of that (adapter, expert)
 // per slice (gate and up are two slices with matrices of their own).
 //
-// The pairs of one (adapter, expert), a group, are multiplied together, 16 at
-// a time (a tile): u = A x over K, split over the workgroup's waves and summed
-// in LDS, then B u over the workgroup's columns, with the 16x16x32 matrix
-// instruction, the matrices as its first operand, so that a lane's four
-// outputs are four consecutive columns of one pair. Both products are one
-// launch: a workgroup has its tile's u whole, and nothing but the result goes
-// to memory. Bound by the bytes of A and B: with the top-k of hundreds of
-// experts a group has few pairs.
+// The pairs of one (adapter, expert), a group, are multiplied together, a tile
+// of up to 16 or 64 of them at a time: u = A x, K split over the workgroup's
+// waves and summed in LDS, then B u over the workgroup's columns, with the
+// 16x16x32 matrix instruction, the matrices as its first operand. Both products
+// are one launch: a workgroup has its tile's u whole, and nothing but the
+// result goes to memory. Bound by the bytes of A and B (with the top-k of
+// hundreds of experts a group has few pairs) and of the result.
+//
+// Few tiles (decode steps): a workgroup per tile, slice and part of the
+// columns, each of which makes u for itself from a matrix A that the parts
+// read out of one L2. Many tiles: a workgroup per tile of 64 pairs takes both
+// slices, so that A, B and x are read once.
 //
 // u enters the second product as the sum of two values of the operands' type,
 // its rounding and the rounding of what is left, so no more than 2^-16 of it
@@ -20,13 +24,14 @@
 // with full precision, so there a pair's u is first scaled by a power of two
 // that puts its largest value near 2^13, and the result scaled back.
 //
-// Grouping. Up to 64 pairs every wave groups them itself, a pair per lane.
-// Above, one launch of up to 256 workgroups, each of which owns a range of
+// Grouping. Up to 256 pairs every workgroup groups them itself: by ballots over
+// the bits of the group up to 64, by comparing each pair with all above. More
+// pairs: one launch of up to 256 workgroups, each of which owns a range of
 // groups: it reads every pair's group, counts those of its range and those
 // below it, and writes its part of the list. A tile's place needs no count of
-// the tiles before it: a range with pb pairs and gb groups below it starts at
-// pb / 16 + min(gb, pb), which leaves room for its tiles whatever their
-// sizes; unused places are marked empty.
+// the tiles before it: with tiles of n pairs, a range with pb pairs and gb
+// groups below it starts at pb / n + min(gb, pb), which leaves room for its
+// tiles whatever their sizes; unused places are marked empty.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
@@ -44,10 +49,10 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kTile = 16;             // pairs per tile
-constexpr int kDirectPairs = 64;      // pairs that a wave groups itself
+constexpr int kFrag = 16;             // pairs of a matrix instruction
+constexpr int kWideTile = 64;         // pairs per tile where there are many
+constexpr int kBallotPairs = 64;      // pairs that a wave groups
+constexpr int kDirectPairs = 256;     // pairs that a workgroup groups
 constexpr int kGroupThreads = 1024;
 constexpr int kRangeGroups = 4096;    // groups a grouping workgroup counts in LDS, at most
 constexpr int64_t kMaxGroups = (1 << 20) - 1;
@@ -132,36 +137,86 @@ __device__ __forceinline__ int2 block_scan2(int2 v, int2* s_tot) {
   return make_int2(base.x + in.x - v.x, base.y + in.y - v.y);
 }
 
+// The groups of token t's pairs k0 .. k0 + N - 1 (-1 past topk): all ids
+// requested before any is used.
+template <int N>
+__device__ __forceinline__ void token_groups(const Ids& d, int64_t t, int k0, int (&g)[N]) {
+  const int64_t a = load_id(d.adapter, d.aeb, t);
+  int64_t e[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int k = k0 + i < d.topk ? k0 + i : d.topk - 1;
+    e[i] = d.expert ? load_id(d.expert, d.eeb, t * d.topk + k) : 0;
+  }
+  int slot[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) slot[i] = !d.expert_map ? 0 : (e[i] >= 0 && e[i] < d.experts ? d.expert_map[e[i]] : -1);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const bool known = e[i] >= 0 && e[i] < d.experts;
+    const int own = known && a >= 0 && a < d.adapters ? static_cast<int>(a) * d.experts + static_cast<int>(e[i])
+                                                      : d.adapters * d.experts;
+    const bool listed = k0 + i < d.topk && (!d.expert_map || (slot[i] >= 0 && slot[i] < d.slots));
+    g[i] = listed ? own : -1;
+  }
+}
+
+// atomicAdd(&cell[g], 1) for the active lanes, in one addition where they all
+// have the same g (the pairs of a dense projection's request come in a row:
+// 64 additions to one LDS word take 64 turns). Returns the lane's own place.
+__device__ __forceinline__ int add_one(int* cell, int g, bool active) {
+  const unsigned long long m = __ballot(active);
+  if (m == 0) return 0;
+  const int lead = __ffsll(static_cast<long long>(m)) - 1;
+  const int g0 = __builtin_amdgcn_readlane(g, lead);
+  if (__ballot(active && g == g0) != m) return active ? atomicAdd(&cell[g], 1) : 0;
+  int at = 0;
+  if (static_cast<int>(threadIdx.x & 63) == lead) at = atomicAdd(&cell[g0], __popcll(m));
+  return __builtin_amdgcn_readlane(at, lead) + static_cast<int>(lane_prefix(m));
+}
+
 // Workgroup w lists the groups [w per, (w + 1) per): pairs[] by group, and a
-// tile entry per kTile pairs of a group.
-__global__ void __launch_bounds__(kGroupThreads) group_kernel(Ids d, int64_t npairs, int per,
+// tile entry per `tile` pairs of a group. A thread takes a token's pairs at a
+// time. The range's own pairs are kept in LDS as they are counted, so that
+// the others are read once; a range with more than kKeep of them reads all
+// pairs again. 65536 pairs of 1537 groups took 108 us pair by pair, each with
+// its division by topk and two round trips of its own, and twice.
+constexpr int kKeep = 4096;
+__global__ void __launch_bounds__(kGroupThreads) group_kernel(Ids d, int64_t tokens, int per, int tile,
                                                               int32_t* __restrict__ pairs,
                                                               Entry* __restrict__ tiles) {
   constexpr int kEach = kRangeGroups / kGroupThreads;
+  constexpr int kAtOnce = 8;
   __shared__ int s_count[kRangeGroups];
+  __shared__ int2 s_keep[kKeep];  // (group less g0, pair)
   __shared__ int2 s_tot[kGroupThreads / 64];
   __shared__ int s_below, s_own;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
   const int groups = d.adapters * d.experts + 1;
   const int g0 = blockIdx.x * per, g1 = g0 + per < groups ? g0 + per : groups;
   for (int i = tid; i < per; i += kGroupThreads) s_count[i] = 0;
   if (tid == 0) s_below = s_own = 0;
   __syncthreads();
-  int below = 0, own = 0;
-  for (int64_t p = tid; p < npairs; p += kGroupThreads) {
-    const int g = pair_group(d, p);
-    if (g < 0) continue;
-    if (g < g0) {
-      ++below;
-    } else if (g < g1) {
-      ++own;
-      atomicAdd(&s_count[g - g0], 1);
+  int below = 0;
+  for (int64_t t = tid; t < tokens; t += kGroupThreads)
+    for (int k0 = 0; k0 < d.topk; k0 += kAtOnce) {
+      int g[kAtOnce];
+      token_groups<kAtOnce>(d, t, k0, g);
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        below += g[i] >= 0 && g[i] < g0;
+        const bool in = g[i] >= g0 && g[i] < g1;
+        if (__ballot(in) == 0) continue;
+        add_one(s_count, g[i] - g0, in);
+        const int at = add_one(&s_own, 0, in);
+        if (in && at < kKeep) s_keep[at] = make_int2(g[i] - g0, static_cast<int>(t * d.topk) + k0 + i);
+      }
     }
-  }
-  atomicAdd(&s_below, below);
-  atomicAdd(&s_own, own);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) below += __shfl_xor(below, off, 64);
+  if (lane == 0 && below) atomicAdd(&s_below, below);
   __syncthreads();
-  const int pb = s_below, all = s_own;
+  const int pb = s_below, own = s_own;
   // A thread's kEach consecutive groups: first pair and first tile.
   int c[kEach];
   int2 mine = make_int2(0, 0);
@@ -170,20 +225,19 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(Ids d, int64_t npa
     const int g = tid * kEach + i;
     c[i] = g < g1 - g0 ? s_count[g] : 0;
     mine.x += c[i];
-    mine.y += (c[i] + kTile - 1) / kTile;
+    mine.y += (c[i] + tile - 1) / tile;
   }
   int2 at = block_scan2(mine, s_tot);  // (a barrier: the counts are read)
-  const int below_groups = g0 < groups ? g0 : groups;
   const int own_groups = g1 > g0 ? g1 - g0 : 0;
-  const int first = pb / kTile + (below_groups < pb ? below_groups : pb);
-  const int upto = below_groups + own_groups, pe = pb + all;
-  const int last = pe / kTile + (upto < pe ? upto : pe);
+  const int first = pb / tile + (g0 < pb ? g0 : pb);
+  const int upto = g0 + own_groups, pe = pb + own;
+  const int last = pe / tile + (upto < pe ? upto : pe);
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int g = tid * kEach + i;
     if (g < g1 - g0) s_count[g] = pb + at.x;  // where the group's next pair goes
-    for (int k = 0; k < c[i]; k += kTile)
-      tiles[first + at.y++] = Entry{g0 + g, pb + at.x + k, c[i] - k < kTile ? c[i] - k : kTile, 0};
+    for (int k = 0; k < c[i]; k += tile)
+      tiles[first + at.y++] = Entry{g0 + g, pb + at.x + k, c[i] - k < tile ? c[i] - k : tile, 0};
     at.x += c[i];
   }
   __syncthreads();
@@ -192,13 +246,30 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(Ids d, int64_t npa
   for (int i = first + used + tid; i < last; i += kGroupThreads) tiles[i] = Entry{0, 0, 0, 0};
   // The places behind the last range, by the last workgroup.
   if (blockIdx.x == gridDim.x - 1) {
-    const int64_t bound = npairs / kTile + (groups < npairs ? groups : npairs);
+    const int64_t npairs = tokens * d.topk;
+    const int64_t bound = npairs / tile + (groups < npairs ? groups : npairs);
     for (int64_t i = last + tid; i < bound; i += kGroupThreads) tiles[i] = Entry{0, 0, 0, 0};
   }
-  for (int64_t p = tid; p < npairs; p += kGroupThreads) {
-    const int g = pair_group(d, p);
-    if (g >= g0 && g < g1) pairs[atomicAdd(&s_count[g - g0], 1)] = static_cast<int32_t>(p);
+  if (own <= kKeep) {
+    for (int i = tid; i < own; i += kGroupThreads) {
+      const int2 v = s_keep[i];
+      const int at = add_one(s_count, v.x, true);
+      pairs[at] = v.y;
+    }
+    return;
   }
+  for (int64_t t = tid; t < tokens; t += kGroupThreads)
+    for (int k0 = 0; k0 < d.topk; k0 += kAtOnce) {
+      int g[kAtOnce];
+      token_groups<kAtOnce>(d, t, k0, g);
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const bool in = g[i] >= g0 && g[i] < g1;
+        if (__ballot(in) == 0) continue;
+        const int at = add_one(s_count, g[i] - g0, in);
+        if (in) pairs[at] = static_cast<int32_t>(t * d.topk) + k0 + i;
+      }
+    }
 }
 
 struct Apply {
@@ -227,57 +298,99 @@ __device__ __forceinline__ float row16_max(float v) {
   return fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x140, 0xF, 0xF, false)));
 }
 
-// Tile i of up to 64 pairs that are grouped here, by one wave (each does it
-// for itself): the group, and row r's pair in lane r (0 .. 15).
-__device__ __forceinline__ bool direct_tile(const Ids& d, int npairs, int i, int& group, int& count, int& row_pair) {
-  const int lane = threadIdx.x & 63;
-  const int g = lane < npairs ? pair_group(d, lane) : -1;
-  unsigned long long same = __ballot(g >= 0);
-  const int bits = 32 - __clz(d.adapters * d.experts);
-  for (int b = 0; b < bits; ++b) {
-    const bool set = (g >> b) & 1;
-    const unsigned long long m = __ballot(set);
-    same &= set ? m : ~m;
+// Tile i of up to kDirectPairs pairs that are grouped here, by the whole
+// workgroup (of at least kDirectPairs threads): the group, its pairs in s_pair
+// and their number; 0: no such tile. Tiles come in the order of their groups'
+// first pairs, and a group's pairs in order, so every workgroup cuts alike.
+struct DirectShared {
+  int key[kDirectPairs];
+  int sum[kDirectPairs / 64];
+  int group, first, count;
+};
+
+__device__ __forceinline__ int direct_tile(const Ids& d, int npairs, int i, DirectShared& s, int* s_pair, int& group) {
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int g = tid < npairs ? pair_group(d, tid) : -1;
+  int rank, total;
+  if (npairs <= kBallotPairs) {
+    if (tid == 0) s.count = 0;
+    unsigned long long same = __ballot(g >= 0);
+    const int bits = 32 - __clz(d.adapters * d.experts);
+    for (int b = 0; b < bits; ++b) {
+      const bool set = (g >> b) & 1;
+      const unsigned long long m = __ballot(set);
+      same &= set ? m : ~m;
+    }
+    rank = static_cast<int>(lane_prefix(same));
+    total = __popcll(same);
+  } else {
+    if (tid == 0) s.count = 0;
+    if (tid < kDirectPairs) s.key[tid] = g;
+    __syncthreads();
+    rank = total = 0;
+#pragma unroll 8
+    for (int p = 0; p < npairs; p += 4) {  // (the places behind the last pair hold -1)
+      const int4 k = *reinterpret_cast<const int4*>(&s.key[p]);
+      const int a = k.x == g, b = k.y == g, c = k.z == g, e = k.w == g;
+      total += a + b + c + e;
+      rank += (p < tid ? a : 0) + (p + 1 < tid ? b : 0) + (p + 2 < tid ? c : 0) + (p + 3 < tid ? e : 0);
+    }
   }
-  const int rank = static_cast<int>(lane_prefix(same));
-  const int ntile = g >= 0 && rank == 0 ? (__popcll(same) + kTile - 1) / kTile : 0;
+  const int ntile = g >= 0 && rank == 0 ? (total + kFrag - 1) / kFrag : 0;
   int start = 0;
+  if (wave < kDirectPairs / 64) {
+    int all = 0;
 #pragma unroll
-  for (int b = 0; b < 3; ++b) start += static_cast<int>(lane_prefix(__ballot((ntile >> b) & 1))) << b;
-  const unsigned long long own = __ballot(ntile > 0 && start <= i && i < start + ntile);
-  if (own == 0) return false;
-  const int lead = __ffsll(static_cast<long long>(own)) - 1;
-  group = __builtin_amdgcn_readlane(g, lead);
-  const int r0 = (i - __builtin_amdgcn_readlane(start, lead)) * kTile;
-  const int all = __popcll(__ballot(g == group));
-  count = all - r0 < kTile ? all - r0 : kTile;
-  const int r = rank - r0;
-  const bool in = g == group && r >= 0 && r < kTile;
-  // Row r's pair goes to lane r; the other lanes' go to lane 63.
-  row_pair = __builtin_amdgcn_ds_permute(4 * (in ? r : 63), lane);
-  return true;
+    for (int b = 0; b < 5; ++b) {
+      const unsigned long long m = __ballot((ntile >> b) & 1);
+      start += static_cast<int>(lane_prefix(m)) << b;
+      all += __popcll(m) << b;
+    }
+    if (lane == 0) s.sum[wave] = all;
+  }
+  __syncthreads();
+  if (wave < kDirectPairs / 64)
+    for (int w = 0; w < wave; ++w) start += s.sum[w];
+  if (ntile > 0 && start <= i && i < start + ntile) {
+    s.group = g;
+    s.first = (i - start) * kFrag;
+    const int left = total - s.first;
+    s.count = left < kFrag ? left : kFrag;
+  }
+  __syncthreads();
+  group = s.group;
+  const int count = s.count;
+  if (count > 0 && g == group && rank >= s.first && rank < s.first + kFrag) s_pair[rank - s.first] = tid;
+  __syncthreads();
+  return count;
 }
 
-// RB: 16-row blocks of a slice's rank. SPW: slices per workgroup.
-template <typename T, int RB, int SPW>
-__global__ void __launch_bounds__(kThreads) lora_kernel(Ids d, Apply p, const int32_t* __restrict__ pairs,
-                                                        const Entry* __restrict__ tiles) {
-  constexpr int NB = RB * SPW, R = 16 * RB;
-  constexpr int kRow = R + 8;  // an LDS row of u: 16 bytes more, so that the rows spread over the banks
-  __shared__ int s_pair[kTile];
-  __shared__ __attribute__((aligned(16))) float s_u[kWaves][NB][16][kTile + 1];
-  __shared__ __attribute__((aligned(16))) uint16_t s_hi[SPW][kTile][kRow], s_lo[SPW][kTile][kRow];
-  __shared__ float s_back[SPW][kTile];
+// RB: 16-row blocks of a slice's rank. SPW: slices per workgroup. MT: 16-pair
+// fragments multiplied at a time. NW: waves.
+template <typename T, int RB, int SPW, int MT, int NW>
+__global__ void __launch_bounds__(64 * NW, NW == 8 ? 4 : 3) lora_kernel(Ids d, Apply p, const int32_t* __restrict__ pairs,
+                                                       const Entry* __restrict__ tiles) {
+  constexpr int NB = RB * SPW, R = 16 * RB, NT = 64 * NW;
+  constexpr int kRow = R + 8;   // an LDS row of u: 16 bytes more, so that the rows spread over the banks
+  constexpr int kPart = 20;     // floats of a pair's 16 ranks in LDS, likewise
+  constexpr int kAhead = NB + MT > 6 ? 1 : NB + MT > 3 ? 2 : 4;  // K steps whose loads are in flight together
+  constexpr bool kEarly = NW == 8;  // B requested before u is made: one workgroup's latency counts, registers do not
+  static_assert(NT >= kDirectPairs, "a thread per pair that is grouped here");
+  __shared__ int s_pair[kWideTile];
+  __shared__ DirectShared s_direct;
+  __shared__ __attribute__((aligned(16))) float s_u[NW][NB * MT][kFrag][kPart];
+  __shared__ __attribute__((aligned(16))) uint16_t s_hi[SPW][MT * kFrag][kRow], s_lo[SPW][MT * kFrag][kRow];
+  __shared__ float s_back[SPW][MT * kFrag];
 
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, j = lane & 15;
-  // Every XCD takes a contiguous part of the tile list, a tile's parts side
-  // by side, so that the tiles of a group read its matrices into one L2.
+  // The tiles are dealt to the XCDs in turn, a tile's parts to one of them, so
+  // that they read its matrices into one L2.
   const int parts = p.slices / SPW * p.nsplit;
-  const int per_xcd = (p.tiles + 7) / 8;
   const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
-  const int ti = xcd * per_xcd + at / parts, part = at % parts;
-  if (at / parts >= per_xcd || ti >= p.tiles) return;
+  const int ti = at / parts * 8 + xcd, part = at % parts;
+  if (ti >= p.tiles) return;
   const int s0 = part / p.nsplit * SPW, split = part % p.nsplit;
 
   int group, count;
@@ -286,24 +399,25 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(Ids d, Apply p, const in
     if (e.count == 0) return;
     group = e.group;
     count = e.count;
-    if (tid < kTile) s_pair[tid] = pairs[e.first + (tid < count ? tid : 0)];
+    if (tid < kWideTile) s_pair[tid] = pairs[e.first + (tid < count ? tid : 0)];
   } else {
-    int row_pair;
-    if (!direct_tile(d, static_cast<int>(p.npairs), ti, group, count, row_pair)) return;
-    const int first = __builtin_amdgcn_readlane(row_pair, 0);
-    if (tid < kTile) s_pair[tid] = tid < count ? row_pair : first;
+    count = direct_tile(d, static_cast<int>(p.npairs), ti, s_direct, s_pair, group);
+    if (count == 0) return;
+    if (tid >= count && tid < kFrag) s_pair[tid] = s_pair[0];
   }
-  __syncthreads();
+  group = __builtin_amdgcn_readfirstlane(group);
+  count = __builtin_amdgcn_readfirstlane(count);
 
-  // This workgroup's 16-column blocks of a slice.
-  const int blocks = p.np / 16, per_split = (blocks + p.nsplit - 1) / p.nsplit;
+  // This workgroup's 32-column blocks of a slice.
+  const int blocks = p.np / 32, per_split = (blocks + p.nsplit - 1) / p.nsplit;
   const int b0 = split * per_split, b1 = b0 + per_split < blocks ? b0 + per_split : blocks;
 
   if (group == d.adapters * d.experts) {  // no adapter: base, or zeros
     if (p.out == p.base) return;
-    const int c0 = b0 * 2, c1 = (b1 * 16 < p.n ? b1 * 16 : p.n) / 8;  // 8-column pieces
+    __syncthreads();
+    const int c0 = b0 * 4, c1 = (b1 * 32 < p.n ? b1 * 32 : p.n) / 8;  // 8-column pieces
     for (int s = s0; s < s0 + SPW; ++s)
-      for (int i = tid; i < count * (c1 - c0); i += kThreads) {
+      for (int i = tid; i < count * (c1 - c0); i += NT) {
         const int r = i / (c1 - c0), c = s * p.n + (c0 + i - r * (c1 - c0)) * 8;
         const int64_t pr = s_pair[r];
         u32x4 v = {0, 0, 0, 0};
@@ -315,44 +429,106 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(Ids d, Apply p, const in
   const int adapter = group / d.experts;
   int rank = p.ranks[adapter];
   rank = rank < 0 ? 0 : (rank < R ? rank : R);
-
-  // u = A x: wave w takes the K steps w, w + 4, ...
-  const int my_pair = s_pair[j];
-  const uint16_t* xrow = p.x + (p.per_pair ? my_pair : my_pair / d.topk) * p.x_stride;
-  const uint16_t* arow = p.a + ((static_cast<int64_t>(group) * p.slices + s0) * R + j) * p.Kp + 8 * q;
-  const int live = (rank + 15) / 16;  // blocks of a slice that hold anything
-  f32x4 acc[NB];
-#pragma unroll
-  for (int i = 0; i < NB; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int live = (rank + 15) / 16;  // 16-row blocks of a slice that hold anything
+  const float scale = p.scales[adapter];
   const int steps = static_cast<int>(p.Kp / 32);
-  for (int k = wave; k < steps; k += kWaves) {
-    u32x4 xv = {0, 0, 0, 0};
-    if (32 * k + 8 * q < p.K) xv = *reinterpret_cast<const u32x4*>(xrow + 32 * k + 8 * q);
+  // A's 16 x 32 blocks lie one behind the other in lane order: a load is 1 KB
+  // in a row. (By rows of K values, 16 rows 4 KB apart are all in one channel
+  // of the L2.)
+  // B's rows of 32 columns, kBlocks blocks of a wave at a time, the first ones
+  // requested before u is made.
+  constexpr int KS = RB == 1 ? 1 : RB / 2;
+  constexpr int kBlocks = KS == 1 ? 4 : KS == 2 ? 2 : 1;
+  u32x4 bv[kBlocks][2][KS];
+  auto load_b = [&](int s, int blk0) {
+    const uint16_t* bmat = p.b + (static_cast<int64_t>(group) * p.slices + s0 + s) * p.np * R;
+    // (an offset of the lane in 32 bits, everything else the same for the wave)
+    const uint32_t own = (8 * (j >> 2) + (j & 3)) * R + 8 * (RB == 1 ? q & 1 : q);
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      if (i % RB >= live) continue;
-      const u32x4 av = *reinterpret_cast<const u32x4*>(arow + static_cast<int64_t>(16 * i) * p.Kp + 32 * k);
-      acc[i] = T::mfma(av, xv, acc[i]);
+    for (int i = 0; i < kBlocks; ++i) {
+      const int blk = __builtin_amdgcn_readfirstlane(blk0 + i * NW < b1 ? blk0 + i * NW : b1 - 1);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+          if (KS == 1 || 32 * k < rank)
+            bv[i][h][k] =
+                *reinterpret_cast<const u32x4*>(bmat + static_cast<int64_t>(32 * blk + 4 * h) * R + 32 * k + own);
     }
-  }
+  };
+  const uint16_t* ablk = p.a + (static_cast<int64_t>(group) * p.slices + s0) * R * p.Kp;
+  const uint32_t alane = 8 * lane;
+
+#pragma unroll 1
+  for (int m0 = 0; m0 < count; m0 += MT * kFrag) {
+    const int frags = count - m0 < MT * kFrag ? (count - m0 + kFrag - 1) / kFrag : MT;
+    // u = A x: wave w takes the K steps w, w + NW, ..., kAhead of them at a
+    // time, the rows of A (which need no pair) requested first.
+    f32x4 acc[NB][MT];
 #pragma unroll
-  for (int i = 0; i < NB; ++i)
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s_u[wave][i][4 * q + r][j] = acc[i][r];
-  __syncthreads();
-  // The waves' sums, and u in two values: 16 threads per pair.
-  {
-    const int pr = tid >> 4, t16 = tid & 15;
+      for (int m = 0; m < MT; ++m) acc[i][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const uint16_t* xrow[MT];
+    if (kEarly && b0 < b1) load_b(0, b0 + wave);
+#pragma unroll 1
+    for (int k0 = wave; k0 < steps; k0 += NW * kAhead) {
+      u32x4 av[kAhead][NB], xv[kAhead][MT];
 #pragma unroll
-    for (int s = 0; s < SPW; ++s) {
+      for (int u = 0; u < kAhead; ++u) {
+        const int k = __builtin_amdgcn_readfirstlane(k0 + u * NW < steps ? k0 + u * NW : steps - 1);
+#pragma unroll
+        for (int i = 0; i < NB; ++i)  // (a block past the rank reads zeros that nothing uses)
+          if (RB <= 2 || i % RB < live)
+            av[u][i] = *reinterpret_cast<const u32x4*>(ablk + (static_cast<int64_t>(i) * steps + k) * 512 + alane);
+      }
+      if (k0 == wave) {
+        if (m0 == 0) __syncthreads();  // s_pair
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const int pr = s_pair[m0 + (m < frags ? m : 0) * kFrag + j];
+          xrow[m] = p.x + static_cast<int64_t>(p.per_pair ? pr : pr / d.topk) * p.x_stride + 8 * q;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int k = k0 + u * NW;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          xv[u][m] = u32x4{0, 0, 0, 0};
+          if (m < frags && 32 * k + 8 * q < p.K) xv[u][m] = *reinterpret_cast<const u32x4*>(xrow[m] + 32 * k);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (k0 + u * NW >= steps) continue;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          if (RB > 2 && i % RB >= live) continue;
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+            if (m < frags) acc[i][m] = T::mfma(av[u][i], xv[u][m], acc[i][m]);
+        }
+      }
+    }
+    if (wave >= steps && m0 == 0) __syncthreads();  // a wave without a step meets the others at s_pair too
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) *reinterpret_cast<f32x4*>(&s_u[wave][i * MT + m][j][4 * q]) = acc[i][m];
+    __syncthreads();
+    // The waves' sums, and u in two values: 16 threads per pair.
+    for (int sm = tid >> 8; sm < SPW * MT; sm += NT / 256) {
+      const int s = sm / MT, m = sm % MT;
+      const int pr = (tid >> 4) & 15, t16 = tid & 15;
       float u[RB];
       float top = 0.0f;
 #pragma unroll
       for (int i = 0; i < RB; ++i) {
-        float v = s_u[0][s * RB + i][t16][pr];
+        float v = s_u[0][(s * RB + i) * MT + m][pr][t16];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) v += s_u[w][s * RB + i][t16][pr];
-        u[i] = 16 * i + t16 < rank ? v : 0.0f;  // zero columns of A times an infinite x are not zero
+        for (int w = 1; w < NW; ++w) v += s_u[w][(s * RB + i) * MT + m][pr][t16];
+        u[i] = 16 * i + t16 < rank ? v : 0.0f;  // zero rows of A times an infinite x are not zero
         if (fabsf(u[i]) < INFINITY) top = fmaxf(top, fabsf(u[i]));
       }
       float up = 1.0f, back = 1.0f;
@@ -364,66 +540,83 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(Ids d, Apply p, const in
         up = ldexpf(1.0f, 14 - e);
         back = ldexpf(1.0f, e - 14);
       }
-      if (t16 == 0) s_back[s][pr] = back;
+      if (t16 == 0) s_back[s][m * kFrag + pr] = back;
 #pragma unroll
       for (int i = 0; i < RB; ++i) {
         const float v = u[i] * up;
         const uint16_t hi = T::bits(v);
         const float rest = v - T::value(hi);
-        s_hi[s][pr][16 * i + t16] = hi;
-        s_lo[s][pr][16 * i + t16] = fabsf(T::value(hi)) < INFINITY ? T::bits(rest) : 0;
+        s_hi[s][m * kFrag + pr][16 * i + t16] = hi;
+        s_lo[s][m * kFrag + pr][16 * i + t16] = fabsf(T::value(hi)) < INFINITY ? T::bits(rest) : 0;
       }
     }
-  }
-  __syncthreads();
+    __syncthreads();
 
-  // B u for this workgroup's columns.
-  const float scale = p.scales[adapter];
-  const int64_t pr = my_pair;
+    // B u for this workgroup's columns, 32 at a time: row i of the first of
+    // the two instructions is column 8 (i / 4) + i % 4, of the second 4 more,
+    // so that a lane's eight outputs are eight consecutive columns of a pair.
 #pragma unroll
-  for (int s = 0; s < SPW; ++s) {
-    const uint16_t* bmat = p.b + (static_cast<int64_t>(group) * p.slices + s0 + s) * p.np * R;
-    const float f = scale * s_back[s][j];
-    // RB = 1: the lanes of the upper half of the instruction's 32 take what
-    // is left of u, with the same 16 columns of B.
-    constexpr int KS = RB == 1 ? 1 : RB / 2;
-    u32x4 hi[KS], lo[KS];
+    for (int s = 0; s < SPW; ++s) {
+      if (s > 0 || !kEarly) load_b(s, b0 + wave);
+      // RB = 1: the lanes of the upper half of the instruction's 32 take what
+      // is left of u, with the same 16 columns of B.
+      u32x4 hi[MT][KS], lo[MT][KS];
+      float f[MT];
+      int64_t row[MT];
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      if constexpr (RB == 1) {
-        hi[0] = *reinterpret_cast<const u32x4*>(q < 2 ? &s_hi[s][j][8 * q] : &s_lo[s][j][8 * (q - 2)]);
-      } else {
-        hi[k] = *reinterpret_cast<const u32x4*>(&s_hi[s][j][32 * k + 8 * q]);
-        lo[k] = *reinterpret_cast<const u32x4*>(&s_lo[s][j][32 * k + 8 * q]);
-      }
-    }
-    for (int blk = b0 + wave; blk < b1; blk += kWaves) {
-      const uint16_t* brow = bmat + static_cast<int64_t>(16 * blk + j) * R + 8 * (RB == 1 ? q & 1 : q);
-      f32x4 y = {0.f, 0.f, 0.f, 0.f};
+      for (int m = 0; m < MT; ++m) {
+        const int r = m * kFrag + j;
+        f[m] = scale * s_back[s][r];
+        row[m] = s_pair[m0 + (m < frags ? r : j)];
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        if (32 * k >= rank) continue;
-        const u32x4 bv = *reinterpret_cast<const u32x4*>(brow + 32 * k);
-        y = T::mfma(bv, hi[k], y);
-        if constexpr (RB > 1) y = T::mfma(bv, lo[k], y);
-      }
-      const int c = 16 * blk + 4 * q;
-      if (j < count && c < p.n) {
-        const int64_t col = static_cast<int64_t>(s0 + s) * p.n + c;
-        float v[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = y[r] * f;
-        if (p.base) {
-          const u32x2 w = *reinterpret_cast<const u32x2*>(p.base + pr * p.base_stride + col);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] += T::value(static_cast<uint16_t>(w[r >> 1] >> (16 * (r & 1))));
+        for (int k = 0; k < KS; ++k) {
+          if constexpr (RB == 1) {
+            hi[m][0] = *reinterpret_cast<const u32x4*>(q < 2 ? &s_hi[s][r][8 * q] : &s_lo[s][r][8 * (q - 2)]);
+          } else {
+            hi[m][k] = *reinterpret_cast<const u32x4*>(&s_hi[s][r][32 * k + 8 * q]);
+            lo[m][k] = *reinterpret_cast<const u32x4*>(&s_lo[s][r][32 * k + 8 * q]);
+          }
         }
-        u32x2 o;
-        o[0] = T::bits(v[0]) | static_cast<uint32_t>(T::bits(v[1])) << 16;
-        o[1] = T::bits(v[2]) | static_cast<uint32_t>(T::bits(v[3])) << 16;
-        *reinterpret_cast<u32x2*>(p.out + pr * p.out_stride + col) = o;
+      }
+#pragma unroll 1
+      for (int blk0 = b0 + wave; blk0 < b1; blk0 += NW * kBlocks) {
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+          const int blk = blk0 + i * NW;
+          if (blk >= b1) continue;
+          const int c = 32 * blk + 8 * q;
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            if (m >= frags) continue;
+            f32x4 y[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int k = 0; k < KS; ++k) {
+                if (KS > 1 && 32 * k >= rank) continue;
+                y[h] = T::mfma(bv[i][h][k], hi[m][k], y[h]);
+                if constexpr (RB > 1) y[h] = T::mfma(bv[i][h][k], lo[m][k], y[h]);
+              }
+            if (m0 + m * kFrag + j >= count || c >= p.n) continue;
+            const int64_t col = static_cast<int64_t>(s0 + s) * p.n + c;
+            float v[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[r] = y[r >> 2][r & 3] * f[m];
+            if (p.base) {
+              const u32x4 w = *reinterpret_cast<const u32x4*>(p.base + row[m] * p.base_stride + col);
+#pragma unroll
+              for (int r = 0; r < 8; ++r) v[r] += T::value(static_cast<uint16_t>(w[r >> 1] >> (16 * (r & 1))));
+            }
+            u32x4 o;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = T::bits(v[2 * r]) | static_cast<uint32_t>(T::bits(v[2 * r + 1])) << 16;
+            *reinterpret_cast<u32x4*>(p.out + row[m] * p.out_stride + col) = o;
+          }
+        }
+        if (blk0 + NW * kBlocks < b1) load_b(s, blk0 + NW * kBlocks);
       }
     }
+    if (m0 + MT * kFrag < count) __syncthreads();  // s_u, s_hi and s_lo are written again
   }
 }
 
@@ -431,9 +624,20 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(Ids d, Apply p, const in
 
 int64_t align256(int64_t n) { return (n + 255) & ~int64_t(255); }
 
-// Places of the tile list: npairs / 16 + min(groups, npairs), the group of the pairs without an adapter among them.
+// Pairs per tile of a listing: 64 where that still makes a tile or more for
+// every CU, whether by the pairs or by the groups, else 16 (more workgroups).
+// By the sizes alone, so that a listing serves every projection of a call.
+int tile_pairs(int64_t npairs, int64_t adapters, int64_t experts) {
+  return npairs / kWideTile >= 256 || std::min(adapters * experts, npairs) >= 256 ? kWideTile : kFrag;
+}
+
+// Places of the tile list: npairs / tile + min(groups, npairs), the group of
+// the pairs without an adapter among them.
+constexpr int64_t kFillWorkgroups = 512;  // workgroups that a call of few tiles is split into, about
+constexpr int64_t kPartBlocks = 2;        // 32-column blocks of a part, at least
+
 int64_t tile_places(int64_t npairs, int64_t adapters, int64_t experts) {
-  return npairs / kTile + std::min(adapters * experts + 1, npairs);
+  return npairs / tile_pairs(npairs, adapters, experts) + std::min(adapters * experts + 1, npairs);
 }
 
 struct Listing {
@@ -478,13 +682,31 @@ int launch_group(const Ids& d, int64_t npairs, void* work, void* stream) {
   Listing w;
   listing_layout(npairs, d.adapters, d.experts, &w, static_cast<uint8_t*>(work));
   const int64_t groups = static_cast<int64_t>(d.adapters) * d.experts + 1;
-  // More pairs take longer to scatter than to read: more workgroups, each with a part of the groups.
+  // Every workgroup reads all pairs; a part of the groups each makes the rest short.
   int64_t wg = std::min<int64_t>(groups, npairs > 2048 ? 64 : 16);
   wg = std::max(wg, (groups + kRangeGroups - 1) / kRangeGroups);
   const int64_t per = (groups + wg - 1) / wg;
   hipLaunchKernelGGL(group_kernel, dim3(static_cast<unsigned>((groups + per - 1) / per)), dim3(kGroupThreads), 0,
-                     as_stream(stream), d, npairs, static_cast<int>(per), w.pairs, w.tiles);
+                     as_stream(stream), d, npairs / d.topk, static_cast<int>(per),
+                     tile_pairs(npairs, d.adapters, d.experts), w.pairs, w.tiles);
   return check_launch("group_kernel");
+}
+
+// One workgroup's shape for RB 16-row blocks of rank: with many tiles MT
+// fragments and, where the slices allow, two slices, as many as a workgroup's
+// LDS and registers hold (8 sums of 16 x 16); with few, one of each and eight
+// waves, so that K is split further.
+template <typename T, int RB, typename F>
+void pick_shape(bool wide, bool even, F&& go) {
+  constexpr int few = RB <= 4 ? 8 : 4;
+  if constexpr (RB == 1) {
+    if (wide) return even ? go(lora_kernel<T, 1, 2, 4, 4>, 2, 4) : go(lora_kernel<T, 1, 1, 4, 4>, 1, 4);
+  } else if constexpr (RB == 2) {
+    if (wide) return even ? go(lora_kernel<T, 2, 2, 2, 4>, 2, 4) : go(lora_kernel<T, 2, 1, 4, 4>, 1, 4);
+  } else if constexpr (RB == 4) {
+    if (wide) return go(lora_kernel<T, 4, 1, 2, 4>, 1, 4);
+  }
+  return go(lora_kernel<T, RB, 1, 1, few>, 1, few);
 }
 
 }  // namespace
@@ -558,34 +780,44 @@ int xp_lora_apply(const void* x, int dtype, int64_t x_stride, int per_pair, int6
   p.ranks = ranks;
   p.slices = static_cast<int>(slices);
   p.n = static_cast<int>(n);
-  p.np = static_cast<int>((n + 15) / 16 * 16);
+  p.np = static_cast<int>((n + 31) / 32 * 32);
   p.base = static_cast<const uint16_t*>(base);
   p.base_stride = base_stride;
   p.out = static_cast<uint16_t*>(out);
   p.out_stride = out_stride;
   p.npairs = npairs;
-  p.nsplit = 1;
   p.tiles = static_cast<int>(direct ? npairs : tile_places(npairs, adapters, experts));
-  const int64_t grid = (p.tiles + 7) / 8 * 8 * slices * p.nsplit;
-  XP_REQUIRE(grid <= INT32_MAX, "%s: %lld workgroups exceed the launch grid", what, (long long)grid);
-  auto go = [&](auto* kernel) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, as_stream(stream), d, p, w.pairs,
-                       w.tiles);
+  // The tiles that can be there: parts of the columns for the rest of the CUs.
+  const bool wide = !direct && tile_pairs(npairs, adapters, experts) == kWideTile;
+  const int64_t likely = std::max(npairs / (wide ? kWideTile : kFrag), std::min(adapters * experts, npairs));
+  int rc = XP_OK;
+  auto launch = [&](auto* kernel, int spw, int waves) {
+    const int64_t fill = kFillWorkgroups / std::max<int64_t>(1, likely * (slices / spw));
+    p.nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(fill, p.np / 32 / kPartBlocks)));
+    const int64_t grid = (p.tiles + 7) / 8 * 8 * (slices / spw) * p.nsplit;
+    if (grid > INT32_MAX) {
+      rc = fail(XP_E_LIMIT, "%s: %lld workgroups exceed the launch grid", what, (long long)grid);
+      return;
+    }
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(static_cast<unsigned>(64 * waves)), 0, as_stream(stream), d,
+                       p, w.pairs, w.tiles);
   };
   auto by_type = [&](auto type) {
     using V = decltype(type);
+    const bool even = slices % 2 == 0;
     switch (R) {
-      case 16: return go(lora_kernel<V, 1, 1>);
-      case 32: return go(lora_kernel<V, 2, 1>);
-      case 64: return go(lora_kernel<V, 4, 1>);
-      case 96: return go(lora_kernel<V, 6, 1>);
-      default: return go(lora_kernel<V, 8, 1>);
+      case 16: return pick_shape<V, 1>(wide, even, launch);
+      case 32: return pick_shape<V, 2>(wide, even, launch);
+      case 64: return pick_shape<V, 4>(wide, even, launch);
+      case 96: return pick_shape<V, 6>(wide, even, launch);
+      default: return pick_shape<V, 8>(wide, even, launch);
     }
   };
   if (dtype == XP_BFLOAT16)
     by_type(Bf16{});
   else
     by_type(Fp16{});
+  if (rc) return rc;
   return check_launch("lora_kernel");
 }
 

@@ -25,7 +25,7 @@ import torch
 from vllm_expert_pager import _native as nat
 
 MAX_RANK = 128
-DIRECT_PAIRS = 64  # pairs up to which the launch groups them itself (no workspace)
+DIRECT_PAIRS = 256  # pairs up to which the launch groups them itself (no workspace)
 _DTYPES = {torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -57,9 +57,10 @@ class LowRankAdapters:
         self.max_rank, self.dtype = max_rank, dtype
         # Storage: ranks in whole matrix-instruction steps, zeros behind what an adapter has.
         self.rank_rows = 16 if max_rank <= 16 else -(-max_rank // 32) * 32
-        self.a = torch.zeros((adapters, experts, slices, self.rank_rows, -(-in_features // 32) * 32), dtype=dtype,
-                             device=device)
-        self.b = torch.zeros((adapters, experts, slices, -(-n // 16) * 16, self.rank_rows), dtype=dtype, device=device)
+        # A by blocks of 16 ranks and 32 inputs, each in the matrix instruction's lane order.
+        self.a = torch.zeros((adapters, experts, slices, self.rank_rows // 16, -(-in_features // 32), 4, 16, 8),
+                             dtype=dtype, device=device)
+        self.b = torch.zeros((adapters, experts, slices, -(-n // 32) * 32, self.rank_rows), dtype=dtype, device=device)
         self.scales = torch.zeros((adapters,), dtype=torch.float32, device=device)
         self.ranks = torch.zeros((adapters,), dtype=torch.int32, device=device)
 
@@ -81,8 +82,10 @@ class LowRankAdapters:
                              f"{self.slices} slices, {self.in_features} inputs and {self.columns} columns")
         if not 1 <= r <= self.max_rank:
             raise ValueError(f"rank {r} (at most {self.max_rank})")
-        self.a[adapter, :, :, :r, : self.in_features] = a
-        self.a[adapter, :, :, r:] = 0
+        steps = self.a.shape[4]
+        whole = torch.zeros((*lead, self.rank_rows, 32 * steps), dtype=self.dtype, device=self.a.device)
+        whole[:, :, :r, : self.in_features] = a
+        self.a[adapter] = whole.view(*lead, -1, 16, steps, 4, 8).permute(0, 1, 2, 4, 5, 3, 6)
         self.b[adapter, :, :, : self.columns, :r] = b
         self.b[adapter, :, :, :, r:] = 0
         self.scales[adapter] = float(scale)
