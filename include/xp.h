@@ -647,7 +647,7 @@ int64_t xp_lora_workspace_bytes(int64_t npairs, int64_t adapters,
  * workspace: adapter adapter_ids[t], expert topk_ids[p] (null: expert 0). A
  * pair whose adapter or expert is out of range has none. expert_map (nullable,
  * int32[experts]): only pairs whose expert has a slot in [0, slots) are
- * listed at all. One launch. */
+ * listed at all. Two launches. */
 int xp_lora_group(const void* adapter_ids, int adapter_elem_bytes,
                   const void* topk_ids, int topk_elem_bytes, int64_t T,
                   int64_t topk, const int32_t* expert_map, int64_t slots,

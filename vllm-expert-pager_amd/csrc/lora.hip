@@ -26,9 +26,9 @@
 //
 // Grouping. Up to 256 pairs every workgroup groups them itself: by ballots over
 // the bits of the group up to 64, by comparing each pair with all above. More
-// pairs: one launch of up to 256 workgroups, each of which owns a range of
-// groups: it reads every pair's group, counts those of its range and those
-// below it, and writes its part of the list. A tile's place needs no count of
+// pairs: a launch that sorts every 256 of them by range of groups, and one of a
+// workgroup per range, which counts and places the groups of its range. A
+// tile's place needs no count of
 // the tiles before it: with tiles of n pairs, a range with pb pairs and gb
 // groups below it starts at pb / n + min(gb, pb), which leaves room for its
 // tiles whatever their sizes; unused places are marked empty.
@@ -137,105 +137,107 @@ __device__ __forceinline__ int2 block_scan2(int2 v, int2* s_tot) {
   return make_int2(base.x + in.x - v.x, base.y + in.y - v.y);
 }
 
-// The groups of token t's pairs k0 .. k0 + N - 1 (-1 past topk): all ids
-// requested before any is used.
-template <int N>
-__device__ __forceinline__ void token_groups(const Ids& d, int64_t t, int k0, int (&g)[N]) {
-  const int64_t a = load_id(d.adapter, d.aeb, t);
-  int64_t e[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int k = k0 + i < d.topk ? k0 + i : d.topk - 1;
-    e[i] = d.expert ? load_id(d.expert, d.eeb, t * d.topk + k) : 0;
-  }
-  int slot[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) slot[i] = !d.expert_map ? 0 : (e[i] >= 0 && e[i] < d.experts ? d.expert_map[e[i]] : -1);
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const bool known = e[i] >= 0 && e[i] < d.experts;
-    const int own = known && a >= 0 && a < d.adapters ? static_cast<int>(a) * d.experts + static_cast<int>(e[i])
-                                                      : d.adapters * d.experts;
-    const bool listed = k0 + i < d.topk && (!d.expert_map || (slot[i] >= 0 && slot[i] < d.slots));
-    g[i] = listed ? own : -1;
-  }
-}
+// A chunk of kChunk pairs: (group, pair) by range of groups, in any order
+// within a range, and where each range begins.
+constexpr int kChunk = 256;
+constexpr int kRanges = 256;  // ranges of groups, at most: the workgroups of group_kernel
 
-// atomicAdd(&cell[g], 1) for the active lanes, in one addition where they all
-// have the same g (the pairs of a dense projection's request come in a row:
-// 64 additions to one LDS word take 64 turns). Returns the lane's own place.
-__device__ __forceinline__ int add_one(int* cell, int g, bool active) {
-  const unsigned long long m = __ballot(active);
-  if (m == 0) return 0;
-  const int lead = __ffsll(static_cast<long long>(m)) - 1;
-  const int g0 = __builtin_amdgcn_readlane(g, lead);
-  if (__ballot(active && g == g0) != m) return active ? atomicAdd(&cell[g], 1) : 0;
-  int at = 0;
-  if (static_cast<int>(threadIdx.x & 63) == lead) at = atomicAdd(&cell[g0], __popcll(m));
-  return __builtin_amdgcn_readlane(at, lead) + static_cast<int>(lane_prefix(m));
+__global__ void __launch_bounds__(kChunk) chunk_kernel(Ids d, int npairs, int per, int ranges,
+                                                       int2* __restrict__ sorted, int32_t* __restrict__ starts) {
+  __shared__ int s_count[kRanges];
+  __shared__ int s_wave[kChunk / 64];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  s_count[tid] = 0;
+  __syncthreads();
+  const int p = blockIdx.x * kChunk + tid;
+  const int g = p < npairs ? pair_group(d, p) : -1;
+  const int r = g >= 0 ? static_cast<int>(static_cast<unsigned>(g) / static_cast<unsigned>(per)) : 0;
+  const int rank = g >= 0 ? atomicAdd(&s_count[r], 1) : 0;
+  __syncthreads();
+  const int mine = s_count[tid];
+  int in = mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int v = __shfl_up(in, off, 64);
+    if (lane >= off) in += v;
+  }
+  if (lane == 63) s_wave[wave] = in;
+  __syncthreads();
+  int before = in - mine;
+  for (int w = 0; w < wave; ++w) before += s_wave[w];
+  s_count[tid] = before;
+  int32_t* row = starts + static_cast<int64_t>(blockIdx.x) * (ranges + 1);
+  if (tid < ranges) row[tid] = before;
+  if (tid == kRanges - 1) row[ranges] = before + mine;
+  __syncthreads();
+  if (g >= 0) sorted[static_cast<int64_t>(blockIdx.x) * kChunk + s_count[r] + rank] = make_int2(g, p);
 }
 
 // Workgroup w lists the groups [w per, (w + 1) per): pairs[] by group, and a
-// tile entry per `tile` pairs of a group. A thread takes a token's pairs at a
-// time. The range's own pairs are kept in LDS as they are counted, so that
-// the others are read once; a range with more than kKeep of them reads all
-// pairs again. 65536 pairs of 1537 groups took 108 us pair by pair, each with
-// its division by topk and two round trips of its own, and twice.
-constexpr int kKeep = 4096;
-__global__ void __launch_bounds__(kGroupThreads) group_kernel(Ids d, int64_t tokens, int per, int tile,
+// tile entry per `tile` pairs of a group. It reads its range's part of every
+// chunk, 16 lanes a chunk, twice (to count, and to place). The starts of the
+// range in the chunks add up to the pairs of the ranges below. (Reading every
+// pair's group in every workgroup took 34 to 90 us for 65536 pairs, however the
+// own ones were taken out; a CU does not get through so many.)
+__global__ void __launch_bounds__(kGroupThreads) group_kernel(const int2* __restrict__ sorted,
+                                                              const int32_t* __restrict__ starts, int64_t npairs,
+                                                              int groups, int per, int ranges, int tile,
                                                               int32_t* __restrict__ pairs,
                                                               Entry* __restrict__ tiles) {
   constexpr int kEach = kRangeGroups / kGroupThreads;
-  constexpr int kAtOnce = 8;
+  constexpr int kTeam = 16, kTeams = kGroupThreads / kTeam;
   __shared__ int s_count[kRangeGroups];
-  __shared__ int2 s_keep[kKeep];  // (group less g0, pair)
   __shared__ int2 s_tot[kGroupThreads / 64];
   __shared__ int s_below, s_own;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int groups = d.adapters * d.experts + 1;
+  const int tid = threadIdx.x;
   const int g0 = blockIdx.x * per, g1 = g0 + per < groups ? g0 + per : groups;
   for (int i = tid; i < per; i += kGroupThreads) s_count[i] = 0;
   if (tid == 0) s_below = s_own = 0;
   __syncthreads();
-  int below = 0;
-  for (int64_t t = tid; t < tokens; t += kGroupThreads)
-    for (int k0 = 0; k0 < d.topk; k0 += kAtOnce) {
-      int g[kAtOnce];
-      token_groups<kAtOnce>(d, t, k0, g);
-#pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) {
-        below += g[i] >= 0 && g[i] < g0;
-        const bool in = g[i] >= g0 && g[i] < g1;
-        if (__ballot(in) == 0) continue;
-        add_one(s_count, g[i] - g0, in);
-        const int at = add_one(&s_own, 0, in);
-        if (in && at < kKeep) s_keep[at] = make_int2(g[i] - g0, static_cast<int>(t * d.topk) + k0 + i);
-      }
+  const int own_groups = g1 > g0 ? g1 - g0 : 0;
+  const int nchunk = static_cast<int>((npairs + kChunk - 1) / kChunk);
+  // f((group, pair)) for the range's pairs.
+  auto own_pairs = [&](auto&& chunk, auto&& f) {
+#pragma unroll 2
+    for (int c = tid / kTeam; c < nchunk; c += kTeams) {
+      const int32_t* row = starts + static_cast<int64_t>(c) * (ranges + 1) + blockIdx.x;
+      const int lo = row[0], hi = row[1];
+      chunk(lo, hi);
+      for (int i = lo + tid % kTeam; i < hi; i += kTeam) f(sorted[static_cast<int64_t>(c) * kChunk + i]);
     }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) below += __shfl_xor(below, off, 64);
-  if (lane == 0 && below) atomicAdd(&s_below, below);
+  };
+  int below = 0, own = 0;
+  own_pairs(
+      [&](int lo, int hi) {
+        below += lo;
+        own += hi - lo;
+      },
+      [&](int2 v) { atomicAdd(&s_count[v.x - g0], 1); });
+  if (tid % kTeam == 0 && (below | own)) {
+    atomicAdd(&s_below, below);
+    atomicAdd(&s_own, own);
+  }
   __syncthreads();
-  const int pb = s_below, own = s_own;
+  const int pb = s_below;
+  own = s_own;
   // A thread's kEach consecutive groups: first pair and first tile.
   int c[kEach];
   int2 mine = make_int2(0, 0);
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int g = tid * kEach + i;
-    c[i] = g < g1 - g0 ? s_count[g] : 0;
+    c[i] = g < own_groups ? s_count[g] : 0;
     mine.x += c[i];
     mine.y += (c[i] + tile - 1) / tile;
   }
   int2 at = block_scan2(mine, s_tot);  // (a barrier: the counts are read)
-  const int own_groups = g1 > g0 ? g1 - g0 : 0;
   const int first = pb / tile + (g0 < pb ? g0 : pb);
   const int upto = g0 + own_groups, pe = pb + own;
   const int last = pe / tile + (upto < pe ? upto : pe);
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int g = tid * kEach + i;
-    if (g < g1 - g0) s_count[g] = pb + at.x;  // where the group's next pair goes
+    if (g < own_groups) s_count[g] = pb + at.x;  // where the group's next pair goes
     for (int k = 0; k < c[i]; k += tile)
       tiles[first + at.y++] = Entry{g0 + g, pb + at.x + k, c[i] - k < tile ? c[i] - k : tile, 0};
     at.x += c[i];
@@ -246,30 +248,10 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(Ids d, int64_t tok
   for (int i = first + used + tid; i < last; i += kGroupThreads) tiles[i] = Entry{0, 0, 0, 0};
   // The places behind the last range, by the last workgroup.
   if (blockIdx.x == gridDim.x - 1) {
-    const int64_t npairs = tokens * d.topk;
     const int64_t bound = npairs / tile + (groups < npairs ? groups : npairs);
     for (int64_t i = last + tid; i < bound; i += kGroupThreads) tiles[i] = Entry{0, 0, 0, 0};
   }
-  if (own <= kKeep) {
-    for (int i = tid; i < own; i += kGroupThreads) {
-      const int2 v = s_keep[i];
-      const int at = add_one(s_count, v.x, true);
-      pairs[at] = v.y;
-    }
-    return;
-  }
-  for (int64_t t = tid; t < tokens; t += kGroupThreads)
-    for (int k0 = 0; k0 < d.topk; k0 += kAtOnce) {
-      int g[kAtOnce];
-      token_groups<kAtOnce>(d, t, k0, g);
-#pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) {
-        const bool in = g[i] >= g0 && g[i] < g1;
-        if (__ballot(in) == 0) continue;
-        const int at = add_one(s_count, g[i] - g0, in);
-        if (in) pairs[at] = static_cast<int32_t>(t * d.topk) + k0 + i;
-      }
-    }
+  own_pairs([](int, int) {}, [&](int2 v) { pairs[atomicAdd(&s_count[v.x - g0], 1)] = v.y; });
 }
 
 struct Apply {
@@ -396,10 +378,16 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 4 : 3) lora_kernel(Ids d, A
   int group, count;
   if (pairs) {
     const Entry e = tiles[ti];
-    if (e.count == 0) return;
+    // (a listing of other sizes addresses nothing out of range)
+    if (e.count <= 0 || e.count > kWideTile || e.first < 0 || e.first + e.count > p.npairs || e.group < 0 ||
+        e.group > d.adapters * d.experts)
+      return;
     group = e.group;
     count = e.count;
-    if (tid < kWideTile) s_pair[tid] = pairs[e.first + (tid < count ? tid : 0)];
+    if (tid < kWideTile) {
+      const int pr = pairs[e.first + (tid < count ? tid : 0)];
+      s_pair[tid] = pr < 0 ? 0 : (pr < p.npairs ? pr : static_cast<int>(p.npairs - 1));
+    }
   } else {
     count = direct_tile(d, static_cast<int>(p.npairs), ti, s_direct, s_pair, group);
     if (count == 0) return;
@@ -641,17 +629,27 @@ int64_t tile_places(int64_t npairs, int64_t adapters, int64_t experts) {
 }
 
 struct Listing {
+  int2* sorted;     // [chunk][kChunk]
+  int32_t* starts;  // [chunk][ranges + 1]
   int32_t* pairs;
   Entry* tiles;
 };
 
+// Groups per range, of at most kRanges ranges (at most kRangeGroups of the 2^20 groups).
+int64_t range_groups(int64_t groups) { return (groups + kRanges - 1) / kRanges; }
+
 int64_t listing_layout(int64_t npairs, int64_t adapters, int64_t experts, Listing* w, uint8_t* base) {
-  const int64_t sz = align256(npairs * 4);
+  const int64_t groups = adapters * experts + 1, per = range_groups(groups), ranges = (groups + per - 1) / per;
+  const int64_t chunks = (npairs + kChunk - 1) / kChunk;
+  const int64_t sz[4] = {align256(npairs * 8), align256(chunks * (ranges + 1) * 4), align256(npairs * 4),
+                         align256(tile_places(npairs, adapters, experts) * static_cast<int64_t>(sizeof(Entry)))};
   if (w) {
-    w->pairs = reinterpret_cast<int32_t*>(base);
-    w->tiles = reinterpret_cast<Entry*>(base + sz);
+    w->sorted = reinterpret_cast<int2*>(base);
+    w->starts = reinterpret_cast<int32_t*>(base + sz[0]);
+    w->pairs = reinterpret_cast<int32_t*>(base + sz[0] + sz[1]);
+    w->tiles = reinterpret_cast<Entry*>(base + sz[0] + sz[1] + sz[2]);
   }
-  return sz + align256(tile_places(npairs, adapters, experts) * static_cast<int64_t>(sizeof(Entry)));
+  return sz[0] + sz[1] + sz[2] + sz[3];
 }
 
 int check_ids(const char* what, const void* adapter_ids, int aeb, const void* topk_ids, int eb, int64_t T, int64_t topk,
@@ -682,12 +680,13 @@ int launch_group(const Ids& d, int64_t npairs, void* work, void* stream) {
   Listing w;
   listing_layout(npairs, d.adapters, d.experts, &w, static_cast<uint8_t*>(work));
   const int64_t groups = static_cast<int64_t>(d.adapters) * d.experts + 1;
-  // Every workgroup reads all pairs; a part of the groups each makes the rest short.
-  int64_t wg = std::min<int64_t>(groups, npairs > 2048 ? 64 : 16);
-  wg = std::max(wg, (groups + kRangeGroups - 1) / kRangeGroups);
-  const int64_t per = (groups + wg - 1) / wg;
-  hipLaunchKernelGGL(group_kernel, dim3(static_cast<unsigned>((groups + per - 1) / per)), dim3(kGroupThreads), 0,
-                     as_stream(stream), d, npairs / d.topk, static_cast<int>(per),
+  const int per = static_cast<int>(range_groups(groups));
+  const unsigned ranges = static_cast<unsigned>((groups + per - 1) / per);
+  hipLaunchKernelGGL(chunk_kernel, dim3(static_cast<unsigned>((npairs + kChunk - 1) / kChunk)), dim3(kChunk), 0,
+                     as_stream(stream), d, static_cast<int>(npairs), per, static_cast<int>(ranges), w.sorted, w.starts);
+  if (int rc = check_launch("chunk_kernel")) return rc;
+  hipLaunchKernelGGL(group_kernel, dim3(ranges), dim3(kGroupThreads), 0, as_stream(stream), w.sorted, w.starts, npairs,
+                     static_cast<int>(groups), per, static_cast<int>(ranges),
                      tile_pairs(npairs, d.adapters, d.experts), w.pairs, w.tiles);
   return check_launch("group_kernel");
 }
@@ -761,7 +760,7 @@ int xp_lora_apply(const void* x, int dtype, int64_t x_stride, int per_pair, int6
              "%s: row strides %lld, %lld and %lld must be multiples of 8 that hold a row", what, (long long)x_stride,
              (long long)base_stride, (long long)out_stride);
   const bool direct = npairs <= kDirectPairs;
-  Listing w{nullptr, nullptr};
+  Listing w{};
   if (!direct) {
     if (int rc = check_listing(what, npairs, adapters, experts, work, work_bytes)) return rc;
     listing_layout(npairs, adapters, experts, &w, static_cast<uint8_t*>(work));
