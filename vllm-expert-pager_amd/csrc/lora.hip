@@ -24,14 +24,14 @@
 // with full precision, so there a pair's u is first scaled by a power of two
 // that puts its largest value near 2^13, and the result scaled back.
 //
-// Grouping. Up to 256 pairs every workgroup groups them itself: by ballots over
-// the bits of the group up to 64, by comparing each pair with all above. More
-// pairs: a launch that sorts every 256 of them by range of groups, and one of a
-// workgroup per range, which counts and places the groups of its range. A
-// tile's place needs no count of
-// the tiles before it: with tiles of n pairs, a range with pb pairs and gb
-// groups below it starts at pb / n + min(gb, pb), which leaves room for its
-// tiles whatever their sizes; unused places are marked empty.
+// Grouping. Up to 64 pairs every wave groups them itself, up to 256 a workgroup
+// finds the pairs of the same group as the one that its tile is named after.
+// More pairs: a launch that sorts every 256 of them by range of groups, and one
+// of a workgroup per range, which counts and places the groups of its range. A
+// tile's place needs no count of the tiles before it: with tiles of n pairs, a
+// range with pb pairs and gb groups below it starts at pb / n + min(gb, pb),
+// which leaves room for its tiles whatever their sizes; unused places are
+// marked empty.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
@@ -85,20 +85,34 @@ struct Fp16 {
   static constexpr bool kScaled = true;
 };
 
+// n / d for 0 <= n < 2^32 by a multiplication: with m = floor(2^64 / d) + 1 the
+// product's high word is the quotient (a division is some 40 instructions).
+struct Divisor {
+  uint64_t m;  // 0: d = 1
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+    if (m == 0) return n;
+    const uint64_t hi = static_cast<uint64_t>(n) * (m >> 32);
+    return static_cast<uint32_t>((hi + __umulhi(n, static_cast<uint32_t>(m))) >> 32);
+  }
+};
+inline Divisor divisor(int64_t d) { return Divisor{d == 1 ? 0 : ~0ull / static_cast<uint64_t>(d) + 1}; }
+
 struct Ids {
   const void* adapter;
   const void* expert;  // null: expert 0
   int aeb, eeb;
   const int32_t* expert_map;  // null: every pair is listed
   int slots;
-  int topk, adapters, experts;
+  int adapters, experts;
+  Divisor by_topk, by_experts;
+  int64_t topk;
 };
 
 // Pair p's group: adapter * experts + expert, adapters * experts for a pair
 // without an adapter, -1 for one that is not listed.
 __device__ __forceinline__ int pair_group(const Ids& d, int64_t p) {
   const int64_t e = d.expert ? load_id(d.expert, d.eeb, p) : 0;
-  const int64_t a = load_id(d.adapter, d.aeb, static_cast<uint32_t>(p) / static_cast<uint32_t>(d.topk));
+  const int64_t a = load_id(d.adapter, d.aeb, d.by_topk(static_cast<uint32_t>(p)));
   const bool known = e >= 0 && e < d.experts;
   if (d.expert_map) {
     const int s = known ? d.expert_map[e] : -1;
@@ -280,86 +294,86 @@ __device__ __forceinline__ float row16_max(float v) {
   return fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x140, 0xF, 0xF, false)));
 }
 
-// Tile i of up to kDirectPairs pairs that are grouped here, by the whole
-// workgroup (of at least kDirectPairs threads): the group, its pairs in s_pair
-// and their number; 0: no such tile. Tiles come in the order of their groups'
-// first pairs, and a group's pairs in order, so every workgroup cuts alike.
-struct DirectShared {
-  int key[kDirectPairs];
-  int sum[kDirectPairs / 64];
-  int group, first, count;
-};
-
-__device__ __forceinline__ int direct_tile(const Ids& d, int npairs, int i, DirectShared& s, int* s_pair, int& group) {
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int g = tid < npairs ? pair_group(d, tid) : -1;
-  int rank, total;
-  if (npairs <= kBallotPairs) {
-    if (tid == 0) s.count = 0;
-    unsigned long long same = __ballot(g >= 0);
-    const int bits = 32 - __clz(d.adapters * d.experts);
-    for (int b = 0; b < bits; ++b) {
-      const bool set = (g >> b) & 1;
-      const unsigned long long m = __ballot(set);
-      same &= set ? m : ~m;
-    }
-    rank = static_cast<int>(lane_prefix(same));
-    total = __popcll(same);
-  } else {
-    if (tid == 0) s.count = 0;
-    if (tid < kDirectPairs) s.key[tid] = g;
-    __syncthreads();
-    rank = total = 0;
-#pragma unroll 8
-    for (int p = 0; p < npairs; p += 4) {  // (the places behind the last pair hold -1)
-      const int4 k = *reinterpret_cast<const int4*>(&s.key[p]);
-      const int a = k.x == g, b = k.y == g, c = k.z == g, e = k.w == g;
-      total += a + b + c + e;
-      rank += (p < tid ? a : 0) + (p + 1 < tid ? b : 0) + (p + 2 < tid ? c : 0) + (p + 3 < tid ? e : 0);
-    }
+// Tile i of up to kBallotPairs pairs, by every wave for itself, a pair a lane:
+// the lanes of one group are found bit by bit, and the tiles numbered in the
+// order of the groups' first pairs, so that the first places are the live ones.
+// Returns the pairs' number (0: no such tile), row r's pair in lane r.
+__device__ __forceinline__ int ballot_tile(const Ids& d, int npairs, int i, int& group, int& row_pair) {
+  const int lane = threadIdx.x & 63;
+  const int g = lane < npairs ? pair_group(d, lane) : -1;
+  unsigned long long same = __ballot(g >= 0);
+  const int bits = 32 - __clz(d.adapters * d.experts);
+#pragma unroll 1
+  for (int b = 0; b < bits; ++b) {
+    const bool set = (g >> b) & 1;
+    const unsigned long long m = __ballot(set);
+    same &= set ? m : ~m;
   }
-  const int ntile = g >= 0 && rank == 0 ? (total + kFrag - 1) / kFrag : 0;
+  const int rank = static_cast<int>(lane_prefix(same));
+  const int ntile = g >= 0 && rank == 0 ? (__popcll(same) + kFrag - 1) / kFrag : 0;
   int start = 0;
-  if (wave < kDirectPairs / 64) {
-    int all = 0;
 #pragma unroll
-    for (int b = 0; b < 5; ++b) {
-      const unsigned long long m = __ballot((ntile >> b) & 1);
-      start += static_cast<int>(lane_prefix(m)) << b;
-      all += __popcll(m) << b;
-    }
-    if (lane == 0) s.sum[wave] = all;
+  for (int b = 0; b < 3; ++b) start += static_cast<int>(lane_prefix(__ballot((ntile >> b) & 1))) << b;
+  const unsigned long long own = __ballot(ntile > 0 && start <= i && i < start + ntile);
+  if (own == 0) return 0;
+  const int lead = __ffsll(static_cast<long long>(own)) - 1;
+  group = __builtin_amdgcn_readlane(g, lead);
+  const int r0 = (i - __builtin_amdgcn_readlane(start, lead)) * kFrag;
+  const int all = __popcll(__ballot(g == group));
+  const int r = rank - r0;
+  const bool in = g == group && r >= 0 && r < kFrag;
+  // Row r's pair goes to lane r; the other lanes' go to lane 63.
+  row_pair = __builtin_amdgcn_ds_permute(4 * (in ? r : 63), lane);
+  return all - r0 < kFrag ? all - r0 : kFrag;
+}
+
+// Tile i of more pairs, up to kDirectPairs, by the whole workgroup (a thread
+// per pair at least): the tile of pair i, if i is the first, the 17th, ... pair
+// of its group. Only that group matters, so one comparison a thread finds its
+// pairs. (Numbering the tiles took 46 LDS reads a thread for 184 pairs, and 5.2
+// us of 14.) Returns the pairs' number (0: no such tile); the barrier behind
+// s_pair is the caller's.
+__device__ __forceinline__ int direct_tile(const Ids& d, int npairs, int i, unsigned long long* s_mask, int* s_pair,
+                                           int& group) {
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  group = pair_group(d, i);
+  const int g = tid < npairs ? pair_group(d, tid) : -1;
+  const unsigned long long mine = __ballot(g == group && g >= 0);
+  if (lane == 0 && wave < kDirectPairs / 64) s_mask[wave] = mine;
+  if (tid < kFrag) s_pair[tid] = i;  // rows past the count repeat the first
+  __syncthreads();
+  int before = 0, total = 0, own = static_cast<int>(lane_prefix(mine));
+#pragma unroll
+  for (int w = 0; w < kDirectPairs / 64; ++w) {
+    const unsigned long long m = s_mask[w];
+    const int n = __popcll(m);
+    if (w < (i >> 6)) before += n;
+    if (w == (i >> 6)) before += __popcll(m & ((1ull << (i & 63)) - 1));
+    if (w < wave) own += n;
+    total += n;
   }
-  __syncthreads();
-  if (wave < kDirectPairs / 64)
-    for (int w = 0; w < wave; ++w) start += s.sum[w];
-  if (ntile > 0 && start <= i && i < start + ntile) {
-    s.group = g;
-    s.first = (i - start) * kFrag;
-    const int left = total - s.first;
-    s.count = left < kFrag ? left : kFrag;
-  }
-  __syncthreads();
-  group = s.group;
-  const int count = s.count;
-  if (count > 0 && g == group && rank >= s.first && rank < s.first + kFrag) s_pair[rank - s.first] = tid;
-  __syncthreads();
-  return count;
+  if (group < 0 || before % kFrag != 0) return 0;
+  const int r = own - before;
+  if (g == group && r > 0 && r < kFrag) s_pair[r] = tid;
+  return total - before < kFrag ? total - before : kFrag;
 }
 
 // RB: 16-row blocks of a slice's rank. SPW: slices per workgroup. MT: 16-pair
 // fragments multiplied at a time. NW: waves.
 template <typename T, int RB, int SPW, int MT, int NW>
-__global__ void __launch_bounds__(64 * NW, NW == 8 ? 4 : 3) lora_kernel(Ids d, Apply p, const int32_t* __restrict__ pairs,
+__global__ void __launch_bounds__(64 * NW, MT == 1 ? 2 : 3) lora_kernel(Ids d, Apply p, const int32_t* __restrict__ pairs,
                                                        const Entry* __restrict__ tiles) {
   constexpr int NB = RB * SPW, R = 16 * RB, NT = 64 * NW;
   constexpr int kRow = R + 8;   // an LDS row of u: 16 bytes more, so that the rows spread over the banks
   constexpr int kPart = 20;     // floats of a pair's 16 ranks in LDS, likewise
-  constexpr int kAhead = NB + MT > 6 ? 1 : NB + MT > 3 ? 2 : 4;  // K steps whose loads are in flight together
-  constexpr bool kEarly = NW == 8;  // B requested before u is made: one workgroup's latency counts, registers do not
+  // K steps whose loads are in flight together. With few tiles a CU has one
+  // workgroup, whose latencies count and whose registers do not: all its loads
+  // at once, and B's first rows requested before u is made.
+  constexpr bool kFew = MT == 1;
+  constexpr int kAhead = kFew ? (NB > 6 ? 2 : NB > 2 ? 4 : 8) : (NB + MT > 6 ? 1 : NB + MT > 3 ? 2 : 4);
   static_assert(NT >= kDirectPairs, "a thread per pair that is grouped here");
   __shared__ int s_pair[kWideTile];
-  __shared__ DirectShared s_direct;
+  __shared__ unsigned long long s_mask[kDirectPairs / 64];
   __shared__ __attribute__((aligned(16))) float s_u[NW][NB * MT][kFrag][kPart];
   __shared__ __attribute__((aligned(16))) uint16_t s_hi[SPW][MT * kFrag][kRow], s_lo[SPW][MT * kFrag][kRow];
   __shared__ float s_back[SPW][MT * kFrag];
@@ -367,13 +381,11 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 4 : 3) lora_kernel(Ids d, A
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, j = lane & 15;
-  // The tiles are dealt to the XCDs in turn, a tile's parts to one of them, so
-  // that they read its matrices into one L2.
-  const int parts = p.slices / SPW * p.nsplit;
-  const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
-  const int ti = at / parts * 8 + xcd, part = at % parts;
+  // Workgroups go to the XCDs in turn, and the grid's width is a multiple of
+  // 8: a tile's parts (slices, columns) read its matrices into one L2.
+  const int ti = blockIdx.x;
   if (ti >= p.tiles) return;
-  const int s0 = part / p.nsplit * SPW, split = part % p.nsplit;
+  const int s0 = blockIdx.z * SPW, split = blockIdx.y;
 
   int group, count;
   if (pairs) {
@@ -389,9 +401,15 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 4 : 3) lora_kernel(Ids d, A
       s_pair[tid] = pr < 0 ? 0 : (pr < p.npairs ? pr : static_cast<int>(p.npairs - 1));
     }
   } else {
-    count = direct_tile(d, static_cast<int>(p.npairs), ti, s_direct, s_pair, group);
+    if (p.npairs <= kBallotPairs) {
+      int row_pair;
+      count = ballot_tile(d, static_cast<int>(p.npairs), ti, group, row_pair);
+      const int first = __builtin_amdgcn_readlane(row_pair, 0);
+      if (tid < kFrag) s_pair[tid] = tid < count ? row_pair : first;
+    } else {
+      count = direct_tile(d, static_cast<int>(p.npairs), ti, s_mask, s_pair, group);
+    }
     if (count == 0) return;
-    if (tid >= count && tid < kFrag) s_pair[tid] = s_pair[0];
   }
   group = __builtin_amdgcn_readfirstlane(group);
   count = __builtin_amdgcn_readfirstlane(count);
@@ -414,7 +432,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 4 : 3) lora_kernel(Ids d, A
       }
     return;
   }
-  const int adapter = group / d.experts;
+  const int adapter = __builtin_amdgcn_readfirstlane(static_cast<int>(d.by_experts(group)));
   int rank = p.ranks[adapter];
   rank = rank < 0 ? 0 : (rank < R ? rank : R);
   const int live = (rank + 15) / 16;  // 16-row blocks of a slice that hold anything
@@ -458,13 +476,14 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 4 : 3) lora_kernel(Ids d, A
 #pragma unroll
       for (int m = 0; m < MT; ++m) acc[i][m] = f32x4{0.f, 0.f, 0.f, 0.f};
     const uint16_t* xrow[MT];
-    if (kEarly && b0 < b1) load_b(0, b0 + wave);
+    if (kFew && b0 < b1) load_b(0, b0 + wave);
 #pragma unroll 1
     for (int k0 = wave; k0 < steps; k0 += NW * kAhead) {
       u32x4 av[kAhead][NB], xv[kAhead][MT];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const int k = __builtin_amdgcn_readfirstlane(k0 + u * NW < steps ? k0 + u * NW : steps - 1);
+        const int k = k0 + u * NW;
+        if (k >= steps) continue;
 #pragma unroll
         for (int i = 0; i < NB; ++i)  // (a block past the rank reads zeros that nothing uses)
           if (RB <= 2 || i % RB < live)
@@ -475,12 +494,13 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 4 : 3) lora_kernel(Ids d, A
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           const int pr = s_pair[m0 + (m < frags ? m : 0) * kFrag + j];
-          xrow[m] = p.x + static_cast<int64_t>(p.per_pair ? pr : pr / d.topk) * p.x_stride + 8 * q;
+          xrow[m] = p.x + static_cast<int64_t>(p.per_pair ? pr : d.by_topk(pr)) * p.x_stride + 8 * q;
         }
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         const int k = k0 + u * NW;
+        if (k >= steps) continue;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           xv[u][m] = u32x4{0, 0, 0, 0};
@@ -545,7 +565,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 8 ? 4 : 3) lora_kernel(Ids d, A
     // so that a lane's eight outputs are eight consecutive columns of a pair.
 #pragma unroll
     for (int s = 0; s < SPW; ++s) {
-      if (s > 0 || !kEarly) load_b(s, b0 + wave);
+      if (s > 0 || !kFew) load_b(s, b0 + wave);
       // RB = 1: the lanes of the upper half of the instruction's 32 take what
       // is left of u, with the same 16 columns of B.
       u32x4 hi[MT][KS], lo[MT][KS];
@@ -621,7 +641,10 @@ int tile_pairs(int64_t npairs, int64_t adapters, int64_t experts) {
 
 // Places of the tile list: npairs / tile + min(groups, npairs), the group of
 // the pairs without an adapter among them.
-constexpr int64_t kFillWorkgroups = 512;  // workgroups that a call of few tiles is split into, about
+// Workgroups that a call of few tiles is split into, about. Every part of a
+// tile's columns reads A for itself: the parts share an L2, which gives about
+// 20 CUs what each can take, so beyond some 160 workgroups they wait for it.
+constexpr int64_t kFillWorkgroups = 160;
 constexpr int64_t kPartBlocks = 2;        // 32-column blocks of a part, at least
 
 int64_t tile_places(int64_t npairs, int64_t adapters, int64_t experts) {
@@ -664,8 +687,8 @@ int check_ids(const char* what, const void* adapter_ids, int aeb, const void* to
   XP_REQUIRE(topk_ids || experts == 1, "%s: %lld experts need topk_ids", what, (long long)experts);
   XP_REQUIRE(expert_map == nullptr || (slots >= 0 && slots <= INT32_MAX), "%s: %lld slots", what, (long long)slots);
   XP_REQUIRE(T == 0 || adapter_ids, "%s: null adapter ids", what);
-  *d = Ids{adapter_ids, topk_ids, aeb, eb, expert_map, static_cast<int>(slots), static_cast<int>(topk),
-           static_cast<int>(adapters), static_cast<int>(experts)};
+  *d = Ids{adapter_ids, topk_ids, aeb, eb, expert_map, static_cast<int>(slots),
+           static_cast<int>(adapters), static_cast<int>(experts), divisor(topk), divisor(experts), topk};
   return XP_OK;
 }
 
@@ -789,17 +812,13 @@ int xp_lora_apply(const void* x, int dtype, int64_t x_stride, int per_pair, int6
   // The tiles that can be there: parts of the columns for the rest of the CUs.
   const bool wide = !direct && tile_pairs(npairs, adapters, experts) == kWideTile;
   const int64_t likely = std::max(npairs / (wide ? kWideTile : kFrag), std::min(adapters * experts, npairs));
-  int rc = XP_OK;
   auto launch = [&](auto* kernel, int spw, int waves) {
     const int64_t fill = kFillWorkgroups / std::max<int64_t>(1, likely * (slices / spw));
     p.nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(fill, p.np / 32 / kPartBlocks)));
-    const int64_t grid = (p.tiles + 7) / 8 * 8 * (slices / spw) * p.nsplit;
-    if (grid > INT32_MAX) {
-      rc = fail(XP_E_LIMIT, "%s: %lld workgroups exceed the launch grid", what, (long long)grid);
-      return;
-    }
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(static_cast<unsigned>(64 * waves)), 0, as_stream(stream), d,
-                       p, w.pairs, w.tiles);
+    const dim3 grid(static_cast<unsigned>((p.tiles + 7) / 8 * 8), static_cast<unsigned>(p.nsplit),
+                    static_cast<unsigned>(slices / spw));
+    hipLaunchKernelGGL(kernel, grid, dim3(static_cast<unsigned>(64 * waves)), 0, as_stream(stream), d, p, w.pairs,
+                       w.tiles);
   };
   auto by_type = [&](auto type) {
     using V = decltype(type);
@@ -816,7 +835,6 @@ int xp_lora_apply(const void* x, int dtype, int64_t x_stride, int per_pair, int6
     by_type(Bf16{});
   else
     by_type(Fp16{});
-  if (rc) return rc;
   return check_launch("lora_kernel");
 }
 
