@@ -172,6 +172,8 @@ def test_refusals():
         with pytest.raises(ValueError):
             call(made)
     good = lora.ExpertAdapters(down=S(1, E, I, H, 4))
+    none = moe.fused_moe(x[:0], tw[:0], ids[:0], *dev, adapters=good, adapter_ids=who[:0])
+    assert tuple(none.shape) == (0, H)
     for bad in (None, who[:2], who.cpu(), who.float()):
         with pytest.raises(ValueError):
             call(good, bad)

@@ -141,7 +141,7 @@ def test_any_order_and_any_split(L, E, T, topk, dtype):
     parts = torch.cat([lora.low_rank(x[t : t + step], stack, adapter[t : t + step],
                                      None if experts is None else experts[t : t + step]) for t in some])
     a, b = whole[: parts.shape[0]].double(), parts.double()
-    # sum |B| (|A| |x|) is below 16 x 0.5 x 5 sigma ... taken from the largest matrices' rows
+    # sum |B| (|A| |x|) is at most the largest row sum of B times that of A times the largest |x|
     reach = max(float(m[2]) * m[1].double().abs().sum(-1).max().item() * m[0].double().abs().sum(-1).max().item()
                 for m in mats) * x.double().abs().max().item()
     assert ((a - b).abs() <= 2 * HALF[dtype] * 1.01 * torch.maximum(a.abs(), b.abs()) + 4 * (K + 16) * U * reach).all()
@@ -224,7 +224,7 @@ def test_no_tokens():
     assert tuple(lora.low_rank(x, stack, ids[:, 0].contiguous(), ids).shape) == (0, 16)
 
 
-@pytest.mark.parametrize("T", [4, 100])
+@pytest.mark.parametrize("T", [4, 100, 200])
 def test_graph_and_stream(T):
     """Captured and replayed on changed tokens, adapters and experts; a call on a side stream."""
     lora = _lora()
@@ -293,3 +293,21 @@ def test_refusals():
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was taken")
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 values of x and of the result: the last rows get what a call of their own gives."""
+    lora = _lora()
+    g = torch.Generator(device="cuda").manual_seed(8)
+    T, K, n, tail = (1 << 20) + 256, 2048, 2048, 256
+    stack, _ = _stack(2, 1, K, n, [8], 1, torch.bfloat16, 8, 3)
+    x = torch.zeros((T, K), dtype=torch.bfloat16, device="cuda")
+    x[-tail:] = torch.randn((tail, K), generator=g, device="cuda").to(torch.bfloat16)
+    assert x.numel() > 1 << 31
+    who = torch.full((T,), -1, dtype=torch.int32, device="cuda")
+    who[-tail:] = torch.arange(tail, device="cuda") % 3 - 1
+    y = lora.low_rank(x, stack, who)
+    own = lora.low_rank(x[-tail:].contiguous(), stack, who[-tail:].contiguous())
+    d = (y[-tail:].double() - own.double()).abs()
+    assert (d <= 2 * 1.01 * HALF[torch.bfloat16] * own.double().abs() + 1e-4).all()  # other parts of K, one rounding each
+    assert y[: T - tail].abs().max() == 0 and own[who[-tail:] >= 0].abs().sum() > 0

@@ -464,3 +464,60 @@ def test_refusals():
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was taken")
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 logits: the last rows get what a call of their own gives."""
+    router = _router()
+    T, E, k, tail = (1 << 22) + 300, 520, 4, 300
+    z = torch.zeros((T, E), dtype=torch.bfloat16, device="cuda")
+    z[-tail:] = _logits(tail, E, torch.bfloat16, 1).cuda()
+    assert z.numel() > 1 << 31
+    own = z[-tail:].clone().requires_grad_(True)
+    w, ids = router.choose_experts(z, k)
+    w2, ids2 = router.choose_experts(own, k)
+    assert torch.equal(ids[-tail:], ids2) and torch.equal(w[-tail:], w2.detach())
+    small = z[:, :500]  # the form for up to 512 experts, rows apart
+    w, ids = router.choose_experts(small, k)
+    w2, ids2 = router.choose_experts(own.detach()[:, :500], k)
+    assert torch.equal(ids[-tail:], ids2) and torch.equal(w[-tail:], w2)
+    leaf = z.requires_grad_(True)
+    offs = torch.tensor([T - tail, T], dtype=torch.int32, device="cuda")
+    loss, counts = router.balance_loss(leaf, torch.zeros((T, 1), dtype=torch.int32, device="cuda"), seq_offsets=offs)
+    (grad,) = torch.autograd.grad(loss, leaf)
+    loss2, counts2 = router.balance_loss(own, torch.zeros((tail, 1), dtype=torch.int32, device="cuda"))
+    (grad2,) = torch.autograd.grad(loss2, own)
+    assert torch.equal(counts[0], counts2) and torch.equal(grad[-tail:], grad2) and grad[: T - tail].abs().max() == 0
+
+
+def test_a_few_calls_at_once():
+    """Calls on several streams at the same time, each with a workspace of its own."""
+    router = _router()
+    zs = [_logits(2000 + 100 * i, 64, torch.float32, i).cuda() for i in range(4)]
+    want = [router.choose_and_balance(z, 4) for z in zs]
+    streams = [torch.cuda.Stream() for _ in zs]
+    got = []
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got.clear()
+        for z, st in zip(zs, streams):
+            with torch.cuda.stream(st):
+                got.append(router.choose_and_balance(z, 4))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_bias_and_groups_in_one_pass_of_many_experts():
+    """The form of a wave per row in choose_and_balance: bias, groups, more than 512 experts or 16 choices."""
+    router = _router()
+    for E, k, how in ((600, 8, {}), (96, 20, {}), (1024, 4, {"bias": True, "groups": 4, "topk_groups": 2})):
+        how = dict(how)
+        if how.pop("bias", False):
+            how["bias"] = 0.1 * torch.randn((E,), generator=torch.Generator().manual_seed(1)).cuda()
+        leaf = _logits(150, E, torch.bfloat16, E).cuda().requires_grad_(True)
+        w, ids, loss, counts = router.choose_and_balance(leaf, k, **how)
+        w2, ids2 = router.choose_experts(leaf, k, **how)
+        loss2, counts2 = router.balance_loss(leaf, ids2)
+        assert torch.equal(w, w2) and torch.equal(ids, ids2) and torch.equal(loss, loss2)
+        assert torch.equal(counts, counts2) and int(counts.sum()) == 150 * k

@@ -817,14 +817,20 @@ int xp_lora_apply(const void* x, int dtype, int64_t x_stride, int per_pair, int6
   // The tiles that can be there: parts of the columns for the rest of the CUs.
   const bool wide = !direct && tile_pairs(npairs, adapters, experts) == kWideTile;
   const int64_t likely = std::max(npairs / (wide ? kWideTile : kFrag), std::min(adapters * experts, npairs));
+  int rc = XP_OK;
   auto launch = [&](auto* kernel, int spw, int waves) {
     const int64_t fill = kFillWorkgroups / std::max<int64_t>(1, likely * (slices / spw));
     p.nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(fill, p.np / 32 / kPartBlocks)));
     const int round = direct ? 8 : 32;  // the XCDs, and runs of four tiles for each
     const dim3 grid(static_cast<unsigned>((p.tiles + round - 1) / round * round), static_cast<unsigned>(p.nsplit),
                     static_cast<unsigned>(slices / spw));
+    if (static_cast<int64_t>(grid.x) * 64 * waves > UINT32_MAX) {
+      rc = fail(XP_E_LIMIT, "%s: %lld pairs exceed the launch grid", what, (long long)npairs);
+      return;
+    }
     hipLaunchKernelGGL(kernel, grid, dim3(static_cast<unsigned>(64 * waves)), 0, as_stream(stream), d, p, w.pairs,
                        w.tiles);
+    rc = check_launch("lora_kernel");
   };
   auto by_type = [&](auto type) {
     using V = decltype(type);
@@ -841,7 +847,7 @@ int xp_lora_apply(const void* x, int dtype, int64_t x_stride, int per_pair, int6
     by_type(Bf16{});
   else
     by_type(Fp16{});
-  return check_launch("lora_kernel");
+  return rc;
 }
 
 }  // extern "C"

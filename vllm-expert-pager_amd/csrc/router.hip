@@ -31,6 +31,7 @@
 #include <hip/hip_fp16.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "common.h"
@@ -1174,7 +1175,7 @@ int check_pick(const char* what, int64_t E, int64_t topk, int scoring, int64_t g
              (long long)keep, (long long)groups, kMaxGroups, (long long)topk, (long long)E);
   XP_REQUIRE(groups == 1 || E <= kMaxGrouped, "%s: groups over %lld experts (at most %d)", what, (long long)E,
              kMaxGrouped);
-  XP_REQUIRE(scale == scale && scale - scale == 0.0, "%s: scale must be finite", what);
+  XP_REQUIRE(scale >= -FLT_MAX && scale <= FLT_MAX, "%s: scale must be a finite fp32 value", what);
   return XP_OK;
 }
 
@@ -1380,7 +1381,7 @@ int xp_router_backward(const void* logits, int dtype, int64_t T, int64_t E, int6
   XP_REQUIRE(grad_weights == nullptr || topk_ids, "%s: the weights' gradient needs the ids", what);
   XP_REQUIRE((counts == nullptr) == (grad_loss == nullptr) && (counts == nullptr) == (tokens == nullptr),
              "%s: the loss's gradient needs counts, tokens and grad_loss", what);
-  XP_REQUIRE(scale == scale && scale - scale == 0.0, "%s: scale must be finite", what);
+  XP_REQUIRE(scale >= -FLT_MAX && scale <= FLT_MAX, "%s: scale must be a finite fp32 value", what);
   if (T == 0) return XP_OK;
   XP_REQUIRE(grad, "%s: null gradient", what);
   const Pick pk{static_cast<int>(topk), scoring == XP_SCORE_SIGMOID, renormalize != 0, 1, 1, static_cast<float>(scale),

@@ -93,19 +93,24 @@ def _stats(logits: torch.Tensor, num_seqs: int, per_seq: bool):
             torch.empty((), dtype=torch.float32, device=dev))
 
 
+def _fp32(grad: torch.Tensor | None) -> torch.Tensor | None:
+    if grad is None or (grad.dtype == torch.float32 and grad.is_contiguous()):
+        return grad
+    return grad.to(torch.float32).contiguous()
+
+
 def _backward(ctx, grad_weights, grad_loss):
     """The logits' gradient through the weights and the loss (either may be None)."""
-    logits, ids, counts, tokens, mask, offsets = ctx.saved_tensors
     if grad_weights is None and grad_loss is None:
         return None
+    logits, ids, counts, tokens, mask, offsets = ctx.saved_tensors
     T, E = logits.shape
     grad = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
-    gw = None if grad_weights is None else grad_weights.to(torch.float32).contiguous()
-    gl = None if grad_loss is None else grad_loss.to(torch.float32).contiguous()
+    gw, gl = _fp32(grad_weights), _fp32(grad_loss)
     through = gl is not None
     nat.call_on(
         logits, "xp_router_backward", logits.data_ptr(), _DTYPES[logits.dtype], T, E, logits.stride(0), ctx.topk,
-        ctx.scoring, ctx.renormalize, ctx.scale, nat.ptr(mask), nat.ptr(offsets), ctx.num_seqs, nat.ptr(ids),
+        ctx.scoring, ctx.renormalize, ctx.scale, nat.ptr(mask), nat.ptr(offsets), ctx.num_seqs, ids.data_ptr(),
         ids.element_size(), nat.ptr(gw), counts.data_ptr() if through else None,
         tokens.data_ptr() if through else None, nat.ptr(gl), grad.data_ptr(),
     )
