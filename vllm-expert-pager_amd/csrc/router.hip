@@ -81,32 +81,68 @@ __device__ __forceinline__ float wave_max(float v) {
 __device__ __forceinline__ uint32_t wave_max_key(uint32_t v) {
   return wave_reduce32(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
-__device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
-  // The largest high word, then the largest low word among its holders.
-  const uint32_t hi = wave_max_key(static_cast<uint32_t>(v >> 32));
-  const uint32_t lo = wave_max_key(static_cast<uint32_t>(v >> 32) == hi ? static_cast<uint32_t>(v) : 0u);
-  return static_cast<uint64_t>(hi) << 32 | lo;
+// A double's halves moved by a DPP control, or swapped between rows (16) or halves (32) of the wave.
+template <int CTRL>
+__device__ __forceinline__ double move_lanes(double v) {
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v));
+  const uint64_t lo = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(b), CTRL, 0xF, 0xF, false));
+  const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(b >> 32), CTRL, 0xF, 0xF, false));
+  return __longlong_as_double(static_cast<long long>(hi << 32 | lo));
+}
+template <int ROWS, typename Op>
+__device__ __forceinline__ double across(double v, Op op) {
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v));
+  const uint32_t l = static_cast<uint32_t>(b), h = static_cast<uint32_t>(b >> 32);
+  uint64_t x, y;
+  if constexpr (ROWS == 16) {
+    const auto lo = __builtin_amdgcn_permlane16_swap(l, l, false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap(h, h, false, false);
+    x = static_cast<uint64_t>(hi[0]) << 32 | lo[0];
+    y = static_cast<uint64_t>(hi[1]) << 32 | lo[1];
+  } else {
+    const auto lo = __builtin_amdgcn_permlane32_swap(l, l, false, false);
+    const auto hi = __builtin_amdgcn_permlane32_swap(h, h, false, false);
+    x = static_cast<uint64_t>(hi[0]) << 32 | lo[0];
+    y = static_cast<uint64_t>(hi[1]) << 32 | lo[1];
+  }
+  return op(__longlong_as_double(static_cast<long long>(x)), __longlong_as_double(static_cast<long long>(y)));
+}
+template <typename Op>
+__device__ __forceinline__ double wave_reduce64(double v, Op op) {
+  v = op(v, move_lanes<0xB1>(v));
+  v = op(v, move_lanes<0x4E>(v));
+  v = op(v, move_lanes<0x141>(v));
+  v = op(v, move_lanes<0x140>(v));
+  v = across<16>(v, op);
+  return across<32>(v, op);
+}
+__device__ __forceinline__ double wave_max_key(double v) {
+  return wave_reduce64(v, [](double a, double b) { return __builtin_fmax(a, b); });
 }
 __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+  return wave_reduce64(v, [](double a, double b) { return a + b; });
 }
 
-// ---- keys: unsigned numbers in the order of the values; 0: masked ----
+// ---- keys ----
+// A logit's key is an unsigned number in its order (0: masked); a score with a
+// bias is its own key in 64 bits (-inf: masked), whose maximum is one
+// instruction where that of 64-bit integers is five.
 __device__ __forceinline__ uint32_t order_key(float v) {
   if (!(v > -INFINITY)) return 0;  // NaN and -inf
   const uint32_t b = __float_as_uint(v + 0.0f);  // -0 counts as 0
   return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
-__device__ __forceinline__ uint64_t order_key(double v) {
-  if (!(v > -static_cast<double>(INFINITY))) return 0;
-  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
-  return b ^ (b >> 63 ? ~0ull : 0x8000000000000000ull);
+template <typename K>
+__device__ __forceinline__ K masked_key() {
+  if constexpr (std::is_same_v<K, double>)
+    return -static_cast<double>(INFINITY);
+  else
+    return 0;
 }
-__device__ __forceinline__ double key_value(uint64_t k) {
-  return __longlong_as_double(static_cast<long long>(k ^ (k >> 63 ? 0x8000000000000000ull : ~0ull)));
-}
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t smaller(uint32_t a, uint32_t b) { return a > b ? b : a; }
+__device__ __forceinline__ double larger(double a, double b) { return __builtin_fmax(a, b); }
+__device__ __forceinline__ double smaller(double a, double b) { return __builtin_fmin(a, b); }
 
 // ---- a row's logits: masked ones as -inf ----
 // LANES lanes hold a row, VPL consecutive experts each.
@@ -166,68 +202,90 @@ struct Pick {
   const float* bias;
 };
 
-// The round's winner: the largest key's lane and position. Returns its index
-// (-1: every key is masked) and takes it out.
+// The round's winner: the first lane that holds the largest key, and there the
+// first position. Returns its index (-1: every key is masked) and takes it out.
 template <typename K, int VPL>
 __device__ __forceinline__ int take_best(K (&key)[VPL]) {
   const int lane = threadIdx.x & 63;
   K best = key[0];
-  int at = 0;
 #pragma unroll
-  for (int i = 1; i < VPL; ++i)
-    if (key[i] > best) {
-      best = key[i];
-      at = i;
-    }
+  for (int i = 1; i < VPL; ++i) best = larger(best, key[i]);
   const K top = wave_max_key(best);
-  if (top == 0) return -1;
+  if (top == masked_key<K>()) return -1;
   const int w = __ffsll(static_cast<long long>(__ballot(best == top))) - 1;
-  const int v = __builtin_amdgcn_readlane(at, w);
-  if (lane == w) {
+  int at = VPL - 1;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (i == v) key[i] = 0;
-  }
+  for (int i = VPL - 2; i >= 0; --i) at = key[i] == top ? i : at;
+  const int v = __builtin_amdgcn_readlane(at, w);
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) key[i] = lane == w && i == v ? masked_key<K>() : key[i];
   return w * VPL + v;
 }
 
-// Masks the keys of the groups that are not among the best `keep`. s_key: E
-// keys of LDS for this wave.
+// A group's two largest keys, a >= b.
+template <typename K>
+__device__ __forceinline__ void take_two(K& a, K& b, K v) {
+  b = larger(b, smaller(a, v));
+  a = larger(a, v);
+}
+// What a group counts: its largest key, or with a bias the sum of the two largest.
+template <typename K>
+__device__ __forceinline__ K group_worth(K a, K b) {
+  if constexpr (std::is_same_v<K, double>)
+    return b > masked_key<K>() ? a + b : a;
+  else
+    return a;
+}
+
+// Masks the keys of the groups that are not among the best `keep`. A group of
+// 2^n whole lanes (256 experts in 8 groups: 8 lanes) is summed up by steps over
+// its lanes; others through s_key, E keys of LDS for this wave, by a lane each.
 template <typename K, int VPL>
 __device__ __forceinline__ void keep_groups(K (&key)[VPL], int E, const Pick& pk, K* s_key) {
   const int lane = threadIdx.x & 63, size = E / pk.groups;
+  const int span = size / VPL;  // lanes of a group
+  const bool lanes = size % VPL == 0 && (span & (span - 1)) == 0;
+  K worth[1] = {masked_key<K>()};
+  int group_of = lane;  // the group that this lane answers for
+  if (lanes) {
+    K a = key[0], b = masked_key<K>();
 #pragma unroll
-  for (int i = 0; i < VPL; ++i)
-    if (lane * VPL + i < E) s_key[lane * VPL + i] = key[i];
-  __builtin_amdgcn_wave_barrier();
-  K worth[1] = {0};
-  if (lane < pk.groups) {
-    K a = 0, b = 0;  // the group's two largest keys
-    for (int i = 0; i < size; ++i) {
-      const K v = s_key[lane * size + i];
-      if (v > a) {
-        b = a;
-        a = v;
-      } else if (v > b) {
-        b = v;
-      }
+    for (int i = 1; i < VPL; ++i) take_two(a, b, key[i]);
+    for (int d = 1; d < span; d <<= 1) {
+      const K oa = __shfl_xor(a, d, 64), ob = __shfl_xor(b, d, 64);
+      take_two(a, b, oa);
+      b = larger(b, ob);
     }
-    worth[0] = a;
-    if constexpr (sizeof(K) == 8) {
-      if (b != 0) worth[0] = order_key(key_value(a) + key_value(b));
+    if (lane % span == 0 && lane * VPL < E) worth[0] = group_worth(a, b);
+    group_of = lane / span;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (lane * VPL + i < E) s_key[lane * VPL + i] = key[i];
+    __builtin_amdgcn_wave_barrier();
+    if (lane < pk.groups) {
+      K a = masked_key<K>(), b = masked_key<K>();
+      for (int i = 0; i < size; ++i) take_two(a, b, s_key[lane * size + i]);
+      worth[0] = group_worth(a, b);
     }
+    __builtin_amdgcn_wave_barrier();
   }
-  __builtin_amdgcn_wave_barrier();
   uint64_t kept = 0;
   for (int g = 0; g < pk.keep; ++g) {
     const int best = take_best<K, 1>(worth);
     if (best < 0) break;
-    kept |= 1ull << best;
+    kept |= 1ull << __builtin_amdgcn_readlane(group_of, best);
+  }
+  if (lanes) {
+    const bool mine = kept >> (group_of & 63) & 1;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) key[i] = mine ? key[i] : masked_key<K>();
+    return;
   }
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
     const int e = lane * VPL + i;
-    if (e < E && !(kept >> (e / size) & 1)) key[i] = 0;
+    if (e < E && !(kept >> (e / size) & 1)) key[i] = masked_key<K>();
   }
 }
 
@@ -235,7 +293,7 @@ __device__ __forceinline__ void keep_groups(K (&key)[VPL], int E, const Pick& pk
 template <typename T, int VPL, bool WIDE>
 __device__ __forceinline__ void choose_row(const T* __restrict__ row, const float (&z)[VPL], int E, const Pick& pk,
                                            void* s_key, int& id, float& weight) {
-  using K = std::conditional_t<WIDE, uint64_t, uint32_t>;
+  using K = std::conditional_t<WIDE, double, uint32_t>;
   const int lane = threadIdx.x & 63;
   K key[VPL];
   if constexpr (WIDE) {
@@ -253,11 +311,12 @@ __device__ __forceinline__ void choose_row(const T* __restrict__ row, const floa
                               : exp(z[i] == m ? 0.0 : static_cast<double>(z[i]) - static_cast<double>(m));
       sum += score[i];
     }
-    sum = pk.sigmoid ? 1.0 : wave_sum(sum);
+    const double inv = pk.sigmoid ? 1.0 : 1.0 / wave_sum(sum);
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       const int e = lane * VPL + i;
-      key[i] = z[i] > -INFINITY ? order_key(score[i] / sum + static_cast<double>(pk.bias[e])) : 0;
+      const double k = z[i] > -INFINITY ? score[i] * inv + static_cast<double>(pk.bias[e]) : masked_key<double>();
+      key[i] = k > masked_key<double>() ? k : masked_key<double>();  // (a bias may be NaN)
     }
   } else {
 #pragma unroll
@@ -629,10 +688,6 @@ struct Key<float> {
     return o ? __uint_as_float(o >> 31 ? o ^ 0x80000000u : ~o) : -INFINITY;
   }
 };
-__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint32_t smaller(uint32_t a, uint32_t b) { return a > b ? b : a; }
-__device__ __forceinline__ double larger(double a, double b) { return __builtin_fmax(a, b); }
-__device__ __forceinline__ double smaller(double a, double b) { return __builtin_fmin(a, b); }
 
 // A list that rises and falls once, sorted (largest first).
 template <int N, typename K>

@@ -200,9 +200,11 @@ def call(name: str, *args) -> None:
     check(getattr(lib(), name)(*args), name)
 
 
-# The current stream's handle without a Stream object around it.
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+# The current stream's handle and the current device without the objects around
+# them (each costs a small call a microsecond).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def stream() -> int:
@@ -213,8 +215,8 @@ def stream() -> int:
 def call_on(t: torch.Tensor, name: str, *args) -> None:
     """``call`` with the current stream of t's device as the last argument, that device being the current one."""
     device = t.get_device()
-    if device == torch.cuda.current_device():
-        rc = getattr(lib(), name)(*args, _raw_stream(device))
+    if device == _current_device():
+        rc = getattr(_lib or lib(), name)(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
             rc = getattr(lib(), name)(*args, _raw_stream(device))
@@ -223,7 +225,7 @@ def call_on(t: torch.Tensor, name: str, *args) -> None:
 
 
 def require_same_device(t: torch.Tensor, other: torch.Tensor, what: str) -> None:
-    if t.device != other.device:
+    if t.get_device() != other.get_device():
         raise ValueError(f"{what} must be on {other.device} (got {t.device})")
 
 
@@ -232,7 +234,7 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def require_device(t: torch.Tensor, what: str) -> None:
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{what} must be a GPU tensor (got {t.device})")
 
 

@@ -190,11 +190,11 @@ def _ids(t: torch.Tensor, what: str, like: torch.Tensor) -> torch.Tensor:
 
 def _rows(t: torch.Tensor, shape: tuple[int, int], what: str, stack: LowRankAdapters) -> None:
     nat.require_same_device(t, stack.a, what)
-    if t.dtype != stack.dtype or tuple(t.shape) != shape:
+    if t.dtype != stack.dtype or t.shape != shape:
         raise ValueError(f"{what} must be {stack.dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
     # Rows may be apart; each starts on 16 bytes and is consecutive.
-    if t.numel() and (t.stride(1) != 1 or (shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < shape[1]))
-                      or t.data_ptr() % 16):
+    if t.data_ptr() % 16 or not t.is_contiguous() and t.numel() and (
+            t.stride(1) != 1 or (shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < shape[1]))):
         raise ValueError(f"{what} must have consecutive rows that start on 16 bytes, got strides {t.stride()}")
 
 
@@ -239,7 +239,7 @@ def low_rank(
     if base is not None:
         _rows(base, (P, stack.out_features), "base", stack)
     if out is None:
-        out = torch.empty((P, stack.out_features), dtype=stack.dtype, device=stack.a.device)
+        out = stack.a.new_empty((P, stack.out_features))
     else:
         _rows(out, (P, stack.out_features), "out", stack)
     if P:

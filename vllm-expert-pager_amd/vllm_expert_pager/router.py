@@ -31,11 +31,11 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 def _logits(logits: torch.Tensor) -> torch.Tensor:
     nat.require_device(logits, "logits")
-    if logits.dim() != 2 or logits.dtype not in _DTYPES or logits.shape[1] == 0:
+    if logits.dtype not in _DTYPES or logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError(f"logits must be a 2-D float32, bfloat16 or float16 tensor, got {logits.dtype} "
                          f"{tuple(logits.shape)}")
     # Rows may be apart (a slice of a wider projection); within a row they are consecutive.
-    if logits.stride(1) != 1 or logits.stride(0) < logits.shape[1]:
+    if not logits.is_contiguous() and (logits.stride(1) != 1 or logits.stride(0) < logits.shape[1]):
         logits = logits.contiguous()
     return logits
 
@@ -223,7 +223,7 @@ def choose_experts(
     args = (logits, topk, code, bool(renormalize), bias, groups, topk_groups, float(scale), _mask(mask, logits))
     if logits.requires_grad and torch.is_grad_enabled():
         return _Choose.apply(*args)
-    return _choose(*args)  # serving: no graph, and none of its cost (half of a one-token call's host time)
+    return _choose(*args)  # serving: no graph, and none of its cost (a third of a one-token call's host time)
 
 
 def balance_loss(
