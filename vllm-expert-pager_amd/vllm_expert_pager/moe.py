@@ -410,13 +410,16 @@ def _adapted_layer(x, topk_weights, topk_ids, w13, w13_scale, w2, w2_scale, expe
                          "(T, topk)")
     S, I = _slab(x.shape[1], w13, w13_scale, w2, w2_scale)
     slots = min(S, MAX_SLOTS)
+    # Pairs without a slot are written by nothing and must add nothing; with a
+    # slot for every expert there are none (a zero fill: 17 us at 2048 tokens).
+    every = expert_map is None and num_experts <= slots
     if expert_map is None:
         expert_map = torch.arange(num_experts, dtype=torch.int32, device=x.device)
     adapted = lora.adapt(x, adapters, adapter_ids, topk_ids, I, num_experts)
     xq, xs, r = quant_route(x, topk_ids, expert_map, slots)
     r.experts = num_experts
-    # Pairs without a slot are written by nothing and add nothing.
-    contrib = torch.zeros((topk_ids.numel(), x.shape[1]), dtype=torch.bfloat16, device=x.device)
+    make = torch.empty if every else torch.zeros
+    contrib = make((topk_ids.numel(), x.shape[1]), dtype=torch.bfloat16, device=x.device)
     run_experts(xq, xs, topk_weights, w13, w13_scale, w2, w2_scale, r, contrib, activation, adapted)
     return topk_sum(contrib, topk_ids, num_experts)
 
