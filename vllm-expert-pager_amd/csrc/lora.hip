@@ -151,6 +151,20 @@ __device__ __forceinline__ int2 block_scan2(int2 v, int2* s_tot) {
   return make_int2(base.x + in.x - v.x, base.y + in.y - v.y);
 }
 
+// atomicAdd(&cell[g], 1) for the active lanes, those of the first lane's g in one
+// addition: the pairs without an adapter, or a dense projection's, are one
+// group of thousands, and 64 additions to one LDS word take 64 turns. Returns
+// the lane's own place.
+__device__ __forceinline__ int add_one(int* cell, int g) {
+  const int g0 = __builtin_amdgcn_readfirstlane(g);
+  const unsigned long long same = __ballot(g == g0);
+  const int lead = __ffsll(static_cast<long long>(same)) - 1;
+  int at = 0;
+  if (g != g0 || static_cast<int>(threadIdx.x & 63) == lead) at = atomicAdd(&cell[g], g == g0 ? __popcll(same) : 1);
+  const int base = __builtin_amdgcn_readlane(at, lead);
+  return g == g0 ? base + static_cast<int>(lane_prefix(same)) : at;
+}
+
 // A chunk of kChunk pairs: (group, pair) by range of groups, in any order
 // within a range, and where each range begins.
 constexpr int kChunk = 256;
@@ -166,7 +180,8 @@ __global__ void __launch_bounds__(kChunk) chunk_kernel(Ids d, int npairs, int pe
   const int p = blockIdx.x * kChunk + tid;
   const int g = p < npairs ? pair_group(d, p) : -1;
   const int r = g >= 0 ? static_cast<int>(static_cast<unsigned>(g) / static_cast<unsigned>(per)) : 0;
-  const int rank = g >= 0 ? atomicAdd(&s_count[r], 1) : 0;
+  int rank = 0;
+  if (g >= 0) rank = add_one(s_count, r);
   __syncthreads();
   const int mine = s_count[tid];
   int in = mine;
@@ -201,6 +216,7 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(const int2* __rest
   constexpr int kEach = kRangeGroups / kGroupThreads;
   constexpr int kTeam = 16, kTeams = kGroupThreads / kTeam;
   __shared__ int s_count[kRangeGroups];
+  __shared__ int s_begin[kRangeGroups + 1], s_tile[kRangeGroups];  // a group's first pair and tile
   __shared__ int2 s_tot[kGroupThreads / 64];
   __shared__ int s_below, s_own;
   const int tid = threadIdx.x;
@@ -210,23 +226,48 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(const int2* __rest
   __syncthreads();
   const int own_groups = g1 > g0 ? g1 - g0 : 0;
   const int nchunk = static_cast<int>((npairs + kChunk - 1) / kChunk);
-  // f((group, pair)) for the range's pairs.
-  auto own_pairs = [&](auto&& chunk, auto&& f) {
-#pragma unroll 2
-    for (int c = tid / kTeam; c < nchunk; c += kTeams) {
-      const int32_t* row = starts + static_cast<int64_t>(c) * (ranges + 1) + blockIdx.x;
-      const int lo = row[0], hi = row[1];
-      chunk(lo, hi);
-      for (int i = lo + tid % kTeam; i < hi; i += kTeam) f(sorted[static_cast<int64_t>(c) * kChunk + i]);
+  // The range's pairs, a team of kTeam lanes a chunk and kRound chunks of a team
+  // at a time, so that their starts, and then their first pairs, are requested
+  // together. One round covers 65536 pairs, and its pairs stay in registers.
+  constexpr int kRound = 4;
+  const int lane16 = tid % kTeam;
+  int lo[kRound], hi[kRound];
+  int2 v[kRound];
+  auto chunk_of = [&](int c0, int i) { return c0 + tid / kTeam + i * kTeams; };
+  auto load_round = [&](int c0) {
+#pragma unroll
+    for (int i = 0; i < kRound; ++i) {
+      const int c = chunk_of(c0, i);
+      lo[i] = hi[i] = 0;
+      if (c < nchunk) {
+        const int32_t* row = starts + static_cast<int64_t>(c) * (ranges + 1) + blockIdx.x;
+        lo[i] = row[0];
+        hi[i] = row[1];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kRound; ++i)
+      if (lo[i] + lane16 < hi[i]) v[i] = sorted[static_cast<int64_t>(chunk_of(c0, i)) * kChunk + lo[i] + lane16];
+  };
+  auto each_pair = [&](int c0, auto&& f) {
+#pragma unroll
+    for (int i = 0; i < kRound; ++i) {
+      if (lo[i] + lane16 < hi[i]) f(v[i]);
+      for (int k = lo[i] + lane16 + kTeam; k < hi[i]; k += kTeam)
+        f(sorted[static_cast<int64_t>(chunk_of(c0, i)) * kChunk + k]);
     }
   };
+  const bool once = nchunk <= kRound * kTeams;
   int below = 0, own = 0;
-  own_pairs(
-      [&](int lo, int hi) {
-        below += lo;
-        own += hi - lo;
-      },
-      [&](int2 v) { atomicAdd(&s_count[v.x - g0], 1); });
+  for (int c0 = 0; c0 < nchunk; c0 += kRound * kTeams) {
+    load_round(c0);
+#pragma unroll
+    for (int i = 0; i < kRound; ++i) {
+      below += lo[i];
+      own += hi[i] - lo[i];
+    }
+    each_pair(c0, [&](int2 p) { add_one(s_count, p.x - g0); });
+  }
   if (tid % kTeam == 0 && (below | own)) {
     atomicAdd(&s_below, below);
     atomicAdd(&s_own, own);
@@ -251,21 +292,44 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(const int2* __rest
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int g = tid * kEach + i;
-    if (g < own_groups) s_count[g] = pb + at.x;  // where the group's next pair goes
-    for (int k = 0; k < c[i]; k += tile)
-      tiles[first + at.y++] = Entry{g0 + g, pb + at.x + k, c[i] - k < tile ? c[i] - k : tile, 0};
+    if (g < own_groups) {
+      s_count[g] = pb + at.x;  // where the group's next pair goes
+      s_begin[g] = pb + at.x;
+      s_tile[g] = at.y;
+    }
     at.x += c[i];
+    at.y += (c[i] + tile - 1) / tile;
   }
+  if (tid == 0) s_begin[own_groups] = pe;
   __syncthreads();
   int used = 0;
   for (int w = 0; w < kGroupThreads / 64; ++w) used += s_tot[w].y;
+  // Tile t belongs to the last group whose tiles begin at or before it.
+  for (int t = tid; t < used; t += kGroupThreads) {
+    int a = 0, z = own_groups;
+    while (z - a > 1) {
+      const int m = (a + z) >> 1;
+      if (s_tile[m] <= t)
+        a = m;
+      else
+        z = m;
+    }
+    const int from = s_begin[a] + (t - s_tile[a]) * tile, left = s_begin[a + 1] - from;
+    tiles[first + t] = Entry{g0 + a, from, left < tile ? left : tile, 0};
+  }
   for (int i = first + used + tid; i < last; i += kGroupThreads) tiles[i] = Entry{0, 0, 0, 0};
   // The places behind the last range, by the last workgroup.
   if (blockIdx.x == gridDim.x - 1) {
     const int64_t bound = npairs / tile + (groups < npairs ? groups : npairs);
     for (int64_t i = last + tid; i < bound; i += kGroupThreads) tiles[i] = Entry{0, 0, 0, 0};
   }
-  own_pairs([](int, int) {}, [&](int2 v) { pairs[atomicAdd(&s_count[v.x - g0], 1)] = v.y; });
+  for (int c0 = 0; c0 < nchunk; c0 += kRound * kTeams) {
+    if (!once) load_round(c0);
+    each_pair(c0, [&](int2 p) {
+      const int at = add_one(s_count, p.x - g0);
+      pairs[at] = p.y;
+    });
+  }
 }
 
 struct Apply {
