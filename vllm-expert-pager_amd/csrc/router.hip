@@ -962,6 +962,7 @@ struct Back {
   const int32_t* counts;      // null: no loss
   const int32_t* tokens;
   const float* grad_loss;
+  bool count_vec;  // rows of counts start on 16 bytes
 };
 
 // d/dz of a row. With G_i the gradient by the probability p_i (the loss's
@@ -1088,6 +1089,22 @@ __device__ __forceinline__ void store_part(T* __restrict__ row, int E, bool vec,
   }
 }
 
+// The counts of a lane's experts (0 past E).
+template <int VPL>
+__device__ __forceinline__ void load_counts(const int32_t* __restrict__ row, int E, bool vec, float (&v)[VPL]) {
+  const int i0 = static_cast<int>(threadIdx.x & (kRowLanes - 1)) * VPL;
+  if (VPL % 4 == 0 && vec && i0 + VPL <= E) {
+    u32x4 c[VPL / 4 > 0 ? VPL / 4 : 1];
+#pragma unroll
+    for (int i = 0; i < VPL / 4; ++i) c[i] = reinterpret_cast<const u32x4*>(row + i0)[i];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) v[i] = static_cast<float>(static_cast<int32_t>(c[i / 4][i % 4]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) v[i] = i0 + i < E ? static_cast<float>(row[i0 + i]) : 0.0f;
+  }
+}
+
 // backward_kernel with rows of 16 lanes. The chosen experts' own terms are
 // added by the lane that holds the choice, which writes that element again
 // behind the row's store, instead of a search for it among the row's lanes.
@@ -1131,11 +1148,12 @@ __global__ void __launch_bounds__(kThreads) backward_narrow_kernel(Rows r, Pick 
     G[i] = 0.0f;
   }
   if (count) {
+    load_counts<VPL>(count, E, b.count_vec, G);
 #pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (l * VPL + i < E) G[i] = k * static_cast<float>(count[l * VPL + i]);
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) dot = fmaf(G[i], p[i], dot);
+    for (int i = 0; i < VPL; ++i) {
+      G[i] *= k;
+      dot = fmaf(G[i], p[i], dot);
+    }
   }
   // The lane's own choice: its share of the weights, probability and slope.
   float w = 0.0f, pc = 0.0f, slope = 1.0f, own = 0.0f;
@@ -1441,7 +1459,7 @@ int xp_router_backward(const void* logits, int dtype, int64_t T, int64_t E, int6
   XP_REQUIRE(grad, "%s: null gradient", what);
   const Pick pk{static_cast<int>(topk), scoring == XP_SCORE_SIGMOID, renormalize != 0, 1, 1, static_cast<float>(scale),
                 nullptr};
-  const Back b{topk_ids, topk_elem_bytes, grad_weights, counts, tokens, grad_loss};
+  const Back b{topk_ids, topk_elem_bytes, grad_weights, counts, tokens, grad_loss, E % 4 == 0 && aligned16(counts)};
   const bool narrow = narrow_rows(E, topk);
   const int lanes = narrow ? kRowLanes : 64, per_block = narrow ? kBlockRows : kWaves;
   const Rows r = rows_of(c, lanes);
