@@ -429,7 +429,6 @@ __global__ void __launch_bounds__(64 * NW, MT == 1 ? 2 : 3) lora_kernel(Ids d, A
                                                        const Entry* __restrict__ tiles) {
   constexpr int NB = RB * SPW, R = 16 * RB, NT = 64 * NW;
   constexpr int kRow = R + 8;   // an LDS row of u: 16 bytes more, so that the rows spread over the banks
-  constexpr int kPart = 20;     // floats of a pair's 16 ranks in LDS, likewise
   // K steps whose loads are in flight together. With few tiles a CU has one
   // workgroup, whose latencies count and whose registers do not: all its loads
   // at once, and B's first rows requested before u is made.
@@ -438,7 +437,7 @@ __global__ void __launch_bounds__(64 * NW, MT == 1 ? 2 : 3) lora_kernel(Ids d, A
   static_assert(NT >= kDirectPairs, "a thread per pair that is grouped here");
   __shared__ int s_pair[kWideTile];
   __shared__ unsigned long long s_mask[kDirectPairs / 64];
-  __shared__ __attribute__((aligned(16))) float s_u[NW][NB * MT][kFrag][kPart];
+  __shared__ __attribute__((aligned(16))) float s_u[NW][NB * MT][kFrag][16];
   __shared__ __attribute__((aligned(16))) uint16_t s_hi[SPW][MT * kFrag][kRow], s_lo[SPW][MT * kFrag][kRow];
   __shared__ float s_back[SPW][MT * kFrag];
 
@@ -513,17 +512,22 @@ __global__ void __launch_bounds__(64 * NW, MT == 1 ? 2 : 3) lora_kernel(Ids d, A
   // B's rows of 32 columns, kBlocks blocks of a wave at a time, the first ones
   // requested before u is made.
   constexpr int KS = RB == 1 ? 1 : RB / 2;
-  constexpr int kBlocks = KS == 1 ? 4 : KS == 2 ? 2 : 1;
-  u32x4 bv[kBlocks][2][KS];
+  constexpr int kBlocks = RB == 1 && SPW == 1 && !kFew ? 8 : KS == 1 ? 4 : KS == 2 ? 2 : 1;
+  // RB = 1: a row is 32 bytes, half an instruction's; the lanes of the upper half
+  // load the second instruction's rows, and the halves are exchanged where they
+  // are used, so that a load has no row twice (2048 tokens' down 50 -> 46 us).
+  constexpr int kHalves = RB == 1 ? 1 : 2;
+  u32x4 bv[kBlocks][kHalves][KS];
   auto load_b = [&](int s, int blk0) {
     const uint16_t* bmat = p.b + (static_cast<int64_t>(group) * p.slices + s0 + s) * p.np * R;
     // (an offset of the lane in 32 bits, everything else the same for the wave)
-    const uint32_t own = (8 * (j >> 2) + (j & 3)) * R + 8 * (RB == 1 ? q & 1 : q);
+    const uint32_t own =
+        RB == 1 ? (8 * (j >> 2) + (j & 3) + 4 * (q >> 1)) * R + 8 * (q & 1) : (8 * (j >> 2) + (j & 3)) * R + 8 * q;
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i) {
       const int blk = __builtin_amdgcn_readfirstlane(blk0 + i * NW < b1 ? blk0 + i * NW : b1 - 1);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < kHalves; ++h)
 #pragma unroll
         for (int k = 0; k < KS; ++k)
           if (KS == 1 || 32 * k < rank)
@@ -662,6 +666,22 @@ __global__ void __launch_bounds__(64 * NW, MT == 1 ? 2 : 3) lora_kernel(Ids d, A
           const int blk = blk0 + i * NW;
           if (blk >= b1) continue;
           const int c = 32 * blk + 8 * q;
+          u32x4 bw[2][KS];
+          if constexpr (RB == 1) {
+            // Both halves of the wave get the lower half's rows, and the upper's.
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const auto t = __builtin_amdgcn_permlane32_swap(bv[i][0][0][w], bv[i][0][0][w], false, false);
+              bw[0][0][w] = t[0];
+              bw[1][0][w] = t[1];
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+              bw[0][k] = bv[i][0][k];
+              bw[1][k] = bv[i][kHalves - 1][k];
+            }
+          }
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             if (m >= frags) continue;
@@ -671,8 +691,8 @@ __global__ void __launch_bounds__(64 * NW, MT == 1 ? 2 : 3) lora_kernel(Ids d, A
 #pragma unroll
               for (int k = 0; k < KS; ++k) {
                 if (KS > 1 && 32 * k >= rank) continue;
-                y[h] = T::mfma(bv[i][h][k], hi[m][k], y[h]);
-                if constexpr (RB > 1) y[h] = T::mfma(bv[i][h][k], lo[m][k], y[h]);
+                y[h] = T::mfma(bw[h][k], hi[m][k], y[h]);
+                if constexpr (RB > 1) y[h] = T::mfma(bw[h][k], lo[m][k], y[h]);
               }
             if (m0 + m * kFrag + j >= count || c >= p.n) continue;
             const int64_t col = static_cast<int64_t>(s0 + s) * p.n + c;
