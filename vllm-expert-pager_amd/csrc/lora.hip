@@ -723,21 +723,37 @@ int64_t align256(int64_t n) { return (n + 255) & ~int64_t(255); }
 
 // Pairs per tile of a listing: 64 where that still makes a tile or more for
 // every CU, whether by the pairs or by the groups, else 16 (more workgroups).
-// By the sizes alone, so that a listing serves every projection of a call.
+// By the sizes alone, so that a listing serves every projection of a call. us
+// with 64 and with 16: 1024 tokens x 4 of 32 experts (64 groups) 34 and 24, 2048
+// dense tokens of four adapters 34 and 21; gate and up of 8192 tokens x 8 of 256
+// experts with 2, 4, 8 and 16 adapters 96, 109, 132 and 187 and 136, 147, 164
+// and 209, of 2048 tokens with one 32 and 39, with four 57 and 58.
 int tile_pairs(int64_t npairs, int64_t adapters, int64_t experts) {
   return npairs / kWideTile >= 256 || std::min(adapters * experts, npairs) >= 256 ? kWideTile : kFrag;
 }
 
-// Places of the tile list: npairs / tile + min(groups, npairs), the group of
-// the pairs without an adapter among them.
+// The same for a call that makes its own listing, which knows its projection: a
+// single slice of rank 16 gains little from 64 (16 rows of A are soon read) and
+// loses the workgroups. us with 64 and with 16, 256 experts x 8 and four
+// adapters: K = 512, 2048 and 4096, 2048 tokens 46 and 41, 76 and 64, 105 and 86,
+// 8192 tokens 122 and 117, 166 and 160, 223 and 208; 32768 dense tokens of 16
+// adapters 84 and 76, of one 77 and 88. With rank 32 (K = 512, 8192 tokens) 136
+// and 177, dense 96 and 111; rank 64 dense 135 and 191.
+int own_tile_pairs(int64_t npairs, int64_t adapters, int64_t experts, int64_t slices, int64_t R) {
+  return R == 16 && slices % 2 == 1 ? kFrag : tile_pairs(npairs, adapters, experts);
+}
+
 // Workgroups that a call of few tiles is split into, about. Every part of a
 // tile's columns reads A for itself: the parts share an L2, which gives about
-// 20 CUs what each can take, so beyond some 160 workgroups they wait for it.
+// 20 CUs what each can take, so beyond some 160 workgroups they wait for it (64
+// dense tokens of 24 adapters of rank 64: 13.8 us with 160, 23 with 256).
 constexpr int64_t kFillWorkgroups = 160;
 constexpr int64_t kPartBlocks = 2;        // 32-column blocks of a part, at least
 
-int64_t tile_places(int64_t npairs, int64_t adapters, int64_t experts) {
-  return npairs / tile_pairs(npairs, adapters, experts) + std::min(adapters * experts + 1, npairs);
+// Places of the tile list: npairs / tile + min(groups, npairs), the group of
+// the pairs without an adapter among them.
+int64_t tile_places(int64_t npairs, int64_t adapters, int64_t experts, int tile) {
+  return npairs / tile + std::min(adapters * experts + 1, npairs);
 }
 
 struct Listing {
@@ -754,7 +770,7 @@ int64_t listing_layout(int64_t npairs, int64_t adapters, int64_t experts, Listin
   const int64_t groups = adapters * experts + 1, per = range_groups(groups), ranges = (groups + per - 1) / per;
   const int64_t chunks = (npairs + kChunk - 1) / kChunk;
   const int64_t sz[4] = {align256(npairs * 8), align256(chunks * (ranges + 1) * 4), align256(npairs * 4),
-                         align256(tile_places(npairs, adapters, experts) * static_cast<int64_t>(sizeof(Entry)))};
+                         align256(tile_places(npairs, adapters, experts, kFrag) * static_cast<int64_t>(sizeof(Entry)))};
   if (w) {
     w->sorted = reinterpret_cast<int2*>(base);
     w->starts = reinterpret_cast<int32_t*>(base + sz[0]);
@@ -788,7 +804,7 @@ int check_listing(const char* what, int64_t npairs, int64_t adapters, int64_t ex
   return XP_OK;
 }
 
-int launch_group(const Ids& d, int64_t npairs, void* work, void* stream) {
+int launch_group(const Ids& d, int64_t npairs, int tile, void* work, void* stream) {
   Listing w;
   listing_layout(npairs, d.adapters, d.experts, &w, static_cast<uint8_t*>(work));
   const int64_t groups = static_cast<int64_t>(d.adapters) * d.experts + 1;
@@ -798,8 +814,7 @@ int launch_group(const Ids& d, int64_t npairs, void* work, void* stream) {
                      as_stream(stream), d, static_cast<int>(npairs), per, static_cast<int>(ranges), w.sorted, w.starts);
   if (int rc = check_launch("chunk_kernel")) return rc;
   hipLaunchKernelGGL(group_kernel, dim3(ranges), dim3(kGroupThreads), 0, as_stream(stream), w.sorted, w.starts, npairs,
-                     static_cast<int>(groups), per, static_cast<int>(ranges),
-                     tile_pairs(npairs, d.adapters, d.experts), w.pairs, w.tiles);
+                     static_cast<int>(groups), per, static_cast<int>(ranges), tile, w.pairs, w.tiles);
   return check_launch("group_kernel");
 }
 
@@ -841,7 +856,7 @@ int xp_lora_group(const void* adapter_ids, int adapter_elem_bytes, const void* t
     return rc;
   if (T == 0) return XP_OK;
   if (int rc = check_listing("xp_lora_group", T * topk, adapters, experts, work, work_bytes)) return rc;
-  return launch_group(d, T * topk, work, stream);
+  return launch_group(d, T * topk, tile_pairs(T * topk, adapters, experts), work, stream);
 }
 
 int xp_lora_apply(const void* x, int dtype, int64_t x_stride, int per_pair, int64_t T, int64_t topk, int64_t K,
@@ -872,12 +887,15 @@ int xp_lora_apply(const void* x, int dtype, int64_t x_stride, int per_pair, int6
              "%s: row strides %lld, %lld and %lld must be multiples of 8 that hold a row", what, (long long)x_stride,
              (long long)base_stride, (long long)out_stride);
   const bool direct = npairs <= kDirectPairs;
+  const int tile = direct    ? kFrag
+                   : grouped ? tile_pairs(npairs, adapters, experts)
+                             : own_tile_pairs(npairs, adapters, experts, slices, R);
   Listing w{};
   if (!direct) {
     if (int rc = check_listing(what, npairs, adapters, experts, work, work_bytes)) return rc;
     listing_layout(npairs, adapters, experts, &w, static_cast<uint8_t*>(work));
     if (!grouped)
-      if (int rc = launch_group(d, npairs, work, stream)) return rc;
+      if (int rc = launch_group(d, npairs, tile, work, stream)) return rc;
   }
   Apply p{};
   p.x = static_cast<const uint16_t*>(x);
@@ -897,9 +915,9 @@ int xp_lora_apply(const void* x, int dtype, int64_t x_stride, int per_pair, int6
   p.out = static_cast<uint16_t*>(out);
   p.out_stride = out_stride;
   p.npairs = npairs;
-  p.tiles = static_cast<int>(direct ? npairs : tile_places(npairs, adapters, experts));
+  p.tiles = static_cast<int>(direct ? npairs : tile_places(npairs, adapters, experts, tile));
   // The tiles that can be there: parts of the columns for the rest of the CUs.
-  const bool wide = !direct && tile_pairs(npairs, adapters, experts) == kWideTile;
+  const bool wide = tile == kWideTile;
   const int64_t likely = std::max(npairs / (wide ? kWideTile : kFrag), std::min(adapters * experts, npairs));
   int rc = XP_OK;
   auto launch = [&](auto* kernel, int spw, int waves) {
