@@ -115,3 +115,25 @@ def test_layout_of_loaded_adapters(K, n, r, rank_rows):
     assert torch.equal(stack.b[1, :, :, :n, :r], b.bfloat16())
     assert stack.b[1, :, :, n:].abs().sum() == 0 and stack.b[1, :, :, :, r:].abs().sum() == 0
     assert stack.a[0].abs().sum() == 0 and stack.scales.tolist() == [0.0, 0.25] and stack.ranks.tolist() == [0, r]
+
+
+@pytest.mark.parametrize("E, S, fits, bad", [
+    (2, 1, [(2, 1), (2,)], [(1, 2), (), (2, 1, 1)]), (1, 2, [(1, 2), (2,)], [(2, 1), ()]), (1, 1, [(1, 1), (1,), ()], [(1, 1, 1), (2,)]),
+    (2, 3, [(2, 3)], [(3, 2), (6,), (1, 6)]),
+])
+def test_shapes_of_loaded_adapters(E, S, fits, bad):
+    """The experts' and the slices' dimension are left out only where they are 1, and never taken for each other."""
+    stack = lora.LowRankAdapters(1, E, 16, S * 8, 4, slices=S, device="cpu")
+    a, b = torch.randn((E * S, 3, 16)), torch.randn((E * S, 8, 3))
+    stack.load(0, a.view(E, S, 3, 16), b.view(E, S, 8, 3))
+    want = stack.a.clone(), stack.b.clone()
+    for lead in fits:
+        stack.clear(0)
+        stack.load(0, a.view(*lead, 3, 16), b.view(*lead, 8, 3))
+        assert torch.equal(stack.a, want[0]) and torch.equal(stack.b, want[1])
+    for lead in bad:
+        n = 1
+        for d in lead:
+            n *= d
+        with pytest.raises(ValueError):
+            stack.load(0, torch.randn((n, 3, 16)).view(*lead, 3, 16), torch.randn((n, 8, 3)).view(*lead, 8, 3))

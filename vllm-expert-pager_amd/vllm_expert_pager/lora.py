@@ -74,8 +74,10 @@ class LowRankAdapters:
         expert. ``scale`` multiplies its output (alpha / r). On the current stream, as any other copy."""
         self._index(adapter)
         lead = (self.experts, self.slices)
-        a, b = (t.reshape(lead + tuple(t.shape[-2:])) if t.dim() >= 2 and t.numel() == lead[0] * lead[1] * t.shape[-1]
-                * t.shape[-2] else t for t in (a, b))
+        # What may stand before a matrix: both dimensions, or without one (or both) of size 1.
+        leads = {lead, lead[: 1 if lead[1] == 1 else 2], lead[1 if lead[0] == 1 else 0 :], () if lead == (1, 1) else lead}
+        a, b = (t.reshape(lead + tuple(t.shape[-2:])) if tuple(t.shape[:-2]) in leads and t.dim() >= 2 else t
+                for t in (a, b))
         r = a.shape[-2] if a.dim() == 4 else -1
         if tuple(a.shape) != (*lead, r, self.in_features) or tuple(b.shape) != (*lead, self.columns, r):
             raise ValueError(f"adapter matrices {tuple(a.shape)} and {tuple(b.shape)} do not fit {self.experts} experts, "
