@@ -659,7 +659,7 @@ int xp_lora_group(const void* adapter_ids, int adapter_elem_bytes,
  * expert e, row = t, or p with per_pair; one rounding to the type of out. A
  * pair without an adapter gets base. base null: 0. Rows are x_stride,
  * base_stride and out_stride elements apart (multiples of 8); out may be
- * base. Sums and the inner product in fp32 (the inner product enters the
+ * base, with the same stride. Sums and the inner product in fp32 (the inner product enters the
  * second one as a sum of two values of the type). grouped != 0: the workspace
  * holds the listing of xp_lora_group for the same ids and sizes; else the call
  * makes it. Calls of at most 256 pairs group themselves and need no workspace. */

@@ -64,7 +64,7 @@ APPLY = dict(x=P, dtype=1, x_stride=64, per_pair=0, T=4, topk=2, K=64, a=P, b=P,
     dict(K=60), dict(K=0), dict(a=None), dict(b=P + 2), dict(scales=None), dict(ranks=None), dict(adapters=0),
     dict(adapters=1 << 19), dict(slices=0), dict(slices=17), dict(n=12), dict(R=48), dict(R=144), dict(who=None),
     dict(web=2), dict(ids=None), dict(eb=1), dict(base=P + 8, base_stride=32), dict(base=P, base_stride=24), dict(out=None),
-    dict(out_stride=24), dict(out_stride=36), dict(T=129), dict(T=129, work=P, nbytes=64), dict(T=129, work=P + 16, nbytes=1 << 30),
+    dict(out_stride=24), dict(out_stride=36), dict(base=P, base_stride=40), dict(T=129), dict(T=129, work=P, nbytes=64), dict(T=129, work=P + 16, nbytes=1 << 30),
 ])
 def test_apply_refuses(bad):
     _refused("xp_lora_apply", *{**APPLY, **bad}.values())

@@ -886,6 +886,9 @@ int xp_lora_apply(const void* x, int dtype, int64_t x_stride, int per_pair, int6
                  (out_stride >= slices * n || npairs <= 1) && (!base || base_stride >= slices * n || npairs <= 1),
              "%s: row strides %lld, %lld and %lld must be multiples of 8 that hold a row", what, (long long)x_stride,
              (long long)base_stride, (long long)out_stride);
+  XP_REQUIRE(out != base || base_stride == out_stride || npairs <= 1,
+             "%s: rows of out and base, in one place, are %lld and %lld elements apart", what, (long long)out_stride,
+             (long long)base_stride);
   const bool direct = npairs <= kDirectPairs;
   const int tile = direct    ? kFrag
                    : grouped ? tile_pairs(npairs, adapters, experts)

@@ -220,8 +220,9 @@ def low_rank(
     experts (None for a projection of one expert: topk 1); a pair with an id
     outside ``[0, experts)`` gets ``base``. ``x`` has a row per token, or one
     per pair (``T * topk`` rows, the experts' activations). ``out`` may be
-    ``base`` itself; it must not overlap ``x``. Types are the stack's; the
-    result is rounded once.
+    ``base`` itself (the same rows), and must not overlap ``x`` or ``base``
+    otherwise. Types are the stack's; the result is rounded once and carries no
+    gradient.
     """
     nat.require_device(stack.a, "the adapters")
     adapter_ids = _ids(adapter_ids, "adapter_ids", stack.a)
