@@ -521,3 +521,15 @@ def test_bias_and_groups_in_one_pass_of_many_experts():
         loss2, counts2 = router.balance_loss(leaf, ids2)
         assert torch.equal(w, w2) and torch.equal(ids, ids2) and torch.equal(loss, loss2)
         assert torch.equal(counts, counts2) and int(counts.sum()) == 150 * k
+
+
+def test_offsets_of_64_bits():
+    """int64 offsets that 32 bits do not hold are behind (or before) every row."""
+    router = _router()
+    z = _logits(50, 16, torch.float32, 11).cuda()
+    near = torch.tensor([-1, 10, 50], device="cuda")
+    far = torch.tensor([-(2**33) + 7, 10, 2**32 + 3], device="cuda")
+    want = router.choose_and_balance(z, 2, seq_offsets=near)
+    got = router.choose_and_balance(z, 2, seq_offsets=far)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    assert int(got[3].sum()) == 100

@@ -79,7 +79,10 @@ def _offsets(seq_offsets: torch.Tensor | None, logits: torch.Tensor) -> tuple[to
             2 <= seq_offsets.numel() <= 65535):
         raise ValueError("seq_offsets must be a 1-D int32 or int64 tensor of 2 to 65535 entries, got "
                          f"{seq_offsets.dtype} {tuple(seq_offsets.shape)}")
-    return seq_offsets.to(torch.int32).contiguous(), seq_offsets.numel() - 1
+    num_seqs = seq_offsets.numel() - 1
+    if seq_offsets.dtype == torch.int64:  # an offset behind every row stays one
+        seq_offsets = seq_offsets.clamp(-1, 2**31 - 1).to(torch.int32)
+    return seq_offsets.contiguous(), num_seqs
 
 
 def _stats(logits: torch.Tensor, num_seqs: int, per_seq: bool):
