@@ -137,3 +137,16 @@ def test_shapes_of_loaded_adapters(E, S, fits, bad):
             n *= d
         with pytest.raises(ValueError):
             stack.load(0, torch.randn((n, 3, 16)).view(*lead, 3, 16), torch.randn((n, 8, 3)).view(*lead, 8, 3))
+
+
+def test_loaded_parameters_keep_no_graph():
+    """Matrices that are trained elsewhere (parameters) are copied: the stack takes no part in their graph."""
+    stack = lora.LowRankAdapters(2, 3, 16, 8, 4, device="cpu")
+    a, b = torch.nn.Parameter(torch.randn((3, 4, 16))), torch.nn.Parameter(torch.randn((3, 8, 4)))
+    stack.load(1, a, b * 2)
+    for t in (stack.a, stack.b, stack.scales, stack.ranks):
+        assert not t.requires_grad and t.grad_fn is None
+    assert torch.equal(stack.b[1, :, 0, :8, :4], (b * 2).detach().bfloat16())
+    stack.load(1, a, b)
+    stack.clear(0)
+    assert torch.equal(stack.b[1, :, 0, :8, :4], b.detach().bfloat16())

@@ -68,6 +68,7 @@ class LowRankAdapters:
     def device(self) -> torch.device:
         return self.a.device
 
+    @torch.no_grad()  # a copy: matrices that are parameters elsewhere leave no graph in the stack
     def load(self, adapter: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
         """Put an adapter in place: ``a`` ``(experts, slices, r, in_features)`` and ``b`` ``(experts, slices,
         out_features / slices, r)``; without the slices' dimension for one slice, without the experts' for one
