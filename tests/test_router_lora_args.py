@@ -150,3 +150,16 @@ def test_loaded_parameters_keep_no_graph():
     stack.load(1, a, b)
     stack.clear(0)
     assert torch.equal(stack.b[1, :, 0, :8, :4], b.detach().bfloat16())
+
+
+@pytest.mark.parametrize("bad", [
+    torch.zeros((7,), dtype=torch.int32), torch.zeros((0,), dtype=torch.int32), torch.zeros((8,), dtype=torch.int64),
+    torch.zeros((16,), dtype=torch.int32)[::2],
+])
+def test_expert_map_of_an_adapted_chunk(bad):
+    """The kernels read an entry per expert of the adapters: a shorter map, or one of other values, is refused."""
+    stack = lora.LowRankAdapters(2, 8, 16, 8, 4, device="cpu")
+    ids = torch.zeros((3, 2), dtype=torch.int32)
+    batch = lora.AdaptedBatch(lora.ExpertAdapters(down=stack), ids[:, 0].contiguous(), ids, None, None)
+    with pytest.raises(ValueError, match="expert_map"):
+        batch.down(torch.zeros((6, 16), dtype=torch.bfloat16), bad, 8)

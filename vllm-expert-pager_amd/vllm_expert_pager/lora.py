@@ -154,6 +154,10 @@ class AdaptedBatch:
         out = torch.empty((T * topk, stack.out_features), dtype=stack.dtype, device=acts.device)
         listing = self.listing
         if expert_map is not None:
+            nat.require_same_device(expert_map, stack.a, "expert_map")
+            if expert_map.dtype != torch.int32 or not expert_map.is_contiguous() or expert_map.numel() < stack.experts:
+                raise ValueError(f"expert_map must be a contiguous int32 tensor of {stack.experts} entries, got "
+                                 f"{expert_map.dtype} {tuple(expert_map.shape)}")
             listing = group(stack, self.adapter_ids, self.topk_ids, expert_map, slots)
         apply(acts, stack, self.adapter_ids, self.topk_ids, T, topk, True, None, out, expert_map=expert_map, slots=slots,
               listing=listing)

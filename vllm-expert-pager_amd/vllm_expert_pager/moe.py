@@ -193,8 +193,8 @@ def run_experts(
     ``activation`` ("silu" or "gelu") is applied to the gate before the
     product with up. ``adapted`` (``lora.adapt`` of the same call) adds the
     requests' low-rank adapters to the three projections, each term rounded to
-    bf16; ``expert_map``, the one that was routed by, tells a chunk's pairs
-    from the others, which it may leave out.
+    bf16; ``expert_map``, the one that was routed by (int32, an entry per expert),
+    tells a chunk's pairs from the others, which it may leave out.
     """
     act = activation_code(activation)
     T, H = xq.shape
