@@ -533,3 +533,104 @@ def test_offsets_of_64_bits():
     got = router.choose_and_balance(z, 2, seq_offsets=far)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
     assert int(got[3].sum()) == 100
+
+
+# The forms that no case above selects: 9 to 16 chosen of up to 512 experts (lists of 16), 257 to 512 experts (32 a lane of
+# 16), and a wave per row with the sigmoid's loss and with more than 16 chosen.
+FORMS = [
+    # T, E, k, dtype, options
+    (70, 60, 9, torch.bfloat16, {}),
+    (70, 256, 16, torch.float32, {}),
+    (65, 16, 16, torch.float16, {"renorm": False}),
+    (40, 200, 12, torch.float32, {"scoring": "sigmoid", "scale": 2.5}),
+    (33, 384, 10, torch.float32, {}),
+    (33, 512, 8, torch.float16, {"renorm": False}),
+    (129, 512, 10, torch.bfloat16, {}),
+    (5, 300, 16, torch.float32, {"scoring": "sigmoid"}),
+    (37, 511, 16, torch.bfloat16, {"scoring": "sigmoid", "renorm": False}),
+    (1, 257, 1, torch.float32, {}),
+    (30, 512, 17, torch.float32, {"scoring": "sigmoid"}),
+    (21, 700, 33, torch.bfloat16, {}),
+]
+FORM_CALLS = [(*f, cuts) for f, cuts in zip(FORMS, [None, [0, 1, 30, 30, 70], None, [2, 40], [5, 5, 33], None,
+                                                    [0, 100, 129], None, [0, 37], None, None, [3, 10, 21]])]
+
+
+@pytest.mark.parametrize("T, E, k, dtype, how", FORMS)
+def test_choice_of_every_form(T, E, k, dtype, how):
+    """As test_choice, with ties, masked logits and padding among the rows."""
+    logits = _logits(T, E, dtype, 3 * T + E)
+    logits[T // 2] = torch.arange(E).remainder(3).to(dtype)
+    logits[T // 3, ::2] = NEG
+    logits[T // 4, 5:] = math.nan
+    mask = np.random.default_rng(T).random(T) < 0.9
+    how = {"renorm": True, **how}
+    renorm = how.pop("renorm")
+    w, ids = _router().choose_experts(logits.cuda(), k, renormalize=renorm, mask=torch.from_numpy(mask).cuda(), **how)
+    z = logits.double().numpy()
+    rw, rids = _choose_ref(z, k, renorm=renorm, mask=mask, **how)
+    assert np.array_equal(ids.cpu().numpy(), rids)
+    _check_weights(w, rw, z)
+
+
+@pytest.mark.parametrize("T, E, k, dtype, how, cuts", FORM_CALLS)
+def test_balance_of_every_form(T, E, k, dtype, how, cuts):
+    """Choice, loss and counts in one pass, and the gradient through both, with masked logits and padding; then the
+    loss of the same choice as a given one. Bounds as in test_balance and test_choice_gradient, added."""
+    router = _router()
+    how = {"renorm": True, "scoring": "softmax", "scale": 1.0, **how}
+    renorm, scoring, scale = how["renorm"], how["scoring"], how["scale"]
+    logits = _logits(T, E, dtype, 5 * T + E)
+    logits[T // 3, ::2] = NEG
+    logits[T // 4, 5:] = math.nan
+    on = np.random.default_rng(E).random(T) < 0.85
+    at = [0, T] if cuts is None else cuts
+    live_rows = on.copy()
+    live_rows[: at[0]] = False
+    live_rows[at[-1] :] = False
+    leaf = logits.cuda().requires_grad_(True)
+    offs = None if cuts is None else torch.tensor(cuts, dtype=torch.int32, device="cuda")
+    mask = torch.from_numpy(on).cuda()
+    gw, gl = torch.randn((T, k), generator=torch.Generator().manual_seed(2)), 64.0
+    w, ids, loss, counts = router.choose_and_balance(leaf, k, scoring=scoring, renormalize=renorm, scale=scale, mask=mask,
+                                                     seq_offsets=offs)
+    (grad,) = torch.autograd.grad([w, loss], leaf, [gw.cuda(), torch.tensor(gl, device="cuda")])
+    z = logits.double().numpy()
+    rw, rids = _choose_ref(z, k, scoring, renorm, scale=scale, mask=live_rows)
+    assert np.array_equal(ids.cpu().numpy(), rids)
+    _check_weights(w, rw, z)
+    rl, rc, spread = _balance_ref(z, rids, k, scoring, live_rows, at)
+    assert np.array_equal(counts.cpu().numpy().reshape(rc.shape), rc)
+    assert abs(loss.item() - rl) <= rl * (T + 64 + _span(z).max()) * U
+    loss2, counts2 = router.balance_loss(leaf, ids, scoring=scoring, mask=mask, seq_offsets=offs)
+    assert torch.equal(loss, loss2) and torch.equal(counts, counts2)
+    score, p = _score(z, scoring)
+    rows, has = np.arange(T)[:, None], rids >= 0
+    pick = np.where(has, rids, 0)
+    own = np.where(has, score[rows, pick], 0.0)
+    slope = 1 - score[rows, pick] if scoring == "sigmoid" else np.ones((T, k))
+    g = np.where(has, gw.double().numpy() * scale, 0.0)
+    if renorm:
+        own = own / np.maximum(own.sum(1, keepdims=True), 1e-300)
+        term = own * slope * (g - (g * own).sum(1, keepdims=True))
+    else:
+        term = g * own * slope
+    ref, near, full = gl * spread, p.copy(), np.zeros((T, E))
+    for t in range(T):
+        for j in np.flatnonzero(has[t]):
+            near[t, pick[t, j]] = max(near[t, pick[t, j]], own[t, j])
+            if renorm or scoring == "sigmoid":
+                ref[t, pick[t, j]] += term[t, j]
+            else:
+                full[t, pick[t, j]] += g[t, j]
+    if not renorm and scoring == "softmax":
+        ref = ref + p * (full - (full * p).sum(1, keepdims=True))
+    used = max(sum(live_rows[a:b].any() for a, b in zip(at, at[1:])), 1)
+    reach = np.full((T, 1), np.abs(g).max())
+    for b, (a, z1) in enumerate(zip(at, at[1:])):
+        n = max(live_rows[a:z1].sum(), 1)
+        reach[a:z1] += gl * rc[b].max(initial=0) * E / (k * n * n * used)
+    err = np.abs(grad.double().cpu().numpy() - ref)
+    bound = _grad_bound(ref, near, reach, E, dtype)
+    assert (err <= bound).all(), float((err / bound).max())
+    assert (grad.cpu()[~torch.from_numpy(live_rows)] == 0).all()
