@@ -181,3 +181,30 @@ def test_refusals():
         call(None)
     assert same(call(good), moe.fused_moe(x, tw, ids, *dev))  # an adapter that was never loaded
     assert same(call(lora.ExpertAdapters()), moe.fused_moe(x, tw, ids, *dev))
+
+
+@pytest.mark.parametrize("which", ["both", "gate_up", "down"])
+@pytest.mark.parametrize("L, E, T, topk, H, I, rank, act", [(4, 64, 150, 4, 256, 128, 16, "silu"),
+                                                            (5, 64, 120, 4, 384, 256, 30, "gelu")])
+def test_layer_of_many_groups_against_the_oracle(L, E, T, topk, H, I, rank, act, which):
+    """256 groups of (adapter, expert) and more: the adapters' terms by tiles of 64 pairs; one expert that most tokens
+    choose, so that tiles are filled."""
+    _, moe, _ = _mods()
+    rng = np.random.default_rng(L + T)
+    weights = M.random_experts(rng, E, H, I)
+    dev = [torch.from_numpy(a).cuda() for a in weights]
+    made, mats = _adapters(L, E, H, I, rank, T, which)
+    x = torch.from_numpy(rng.standard_normal((T, H)).astype(np.float32)).to(torch.bfloat16).cuda()
+    ids = np.stack([rng.permutation(E)[:topk] for _ in range(T)]).astype(np.int64)
+    ids[:, 1][(ids != 7).all(1)] = 7
+    ids[0, 0] = -1
+    tw = rng.random((T, topk)).astype(np.float32)
+    who = np.where(rng.random(T) < 0.6, 1, rng.integers(-1, L, T)).astype(np.int32)
+    assert L * E >= 256 and ((who == 1)[:, None] & (ids == 7)).sum() > 64
+    args = (x, torch.from_numpy(tw).cuda(), torch.from_numpy(ids).cuda(), *dev)
+    out = moe.fused_moe(*args, activation=act, adapters=made, adapter_ids=torch.from_numpy(who).cuda())
+    ref = _oracle(x.float().cpu().numpy(), tw, ids, who, weights, mats, act)
+    _check_close(out.float().cpu().numpy(), ref, f"{which} L={L} E={E} T={T}")
+    plain = moe.fused_moe(*args, activation=act)
+    none = torch.from_numpy(who < 0).cuda()
+    assert same(out[none], plain[none]) and not same(out[~none], plain[~none])

@@ -311,3 +311,138 @@ def test_offsets_past_32_bits():
     d = (y[-tail:].double() - own.double()).abs()
     assert (d <= 2 * 1.01 * HALF[torch.bfloat16] * own.double().abs() + 1e-4).all()  # other parts of K, one rounding each
     assert y[: T - tail].abs().max() == 0 and own[who[-tail:] >= 0].abs().sum() > 0
+
+
+# Tiles of 64 pairs: listings of 256 groups or of 16384 pairs at least. A call of one slice (or three) of rank 16 that
+# lists for itself takes 16-pair tiles instead, the large cases of test_any_order_and_any_split among them; from a
+# listing of lora.group it gets tiles of 64 too.
+
+GROUP_SIZES = [1, 16, 17, 33, 63, 64, 65, 130]
+
+
+def _grouped_batch(L, E, topk, sizes, seed):
+    """(adapter, ids) whose groups have these sizes; tokens without an adapter and pairs without an expert among them,
+    in random order."""
+    rng = np.random.default_rng(seed)
+    cells = rng.permutation(L * E)[: len(sizes)]
+    adapter, ids = [], []
+    for cell, size in zip(cells, sizes):
+        a, e = divmod(int(cell), E)
+        for left in range(size, 0, -topk):
+            row = [e] * min(left, topk) + [-1] * (topk - min(left, topk))
+            adapter.append(a)
+            ids.append(rng.permutation(row))
+    for a in (-1, L, -1, 0, 0):
+        adapter.append(a)
+        ids.append(rng.integers(0, E, topk) if not 0 <= a < L else np.full(topk, E))
+    order = rng.permutation(len(adapter))
+    return (torch.from_numpy(np.array(adapter)[order]).to(torch.int32).cuda(),
+            torch.from_numpy(np.stack(ids)[order].astype(np.int64)).cuda())
+
+
+def _ref_by_group(x, mats, adapter, ids, slices, n, K, base, per_pair, dtype):
+    """_ref, a group of pairs at a time."""
+    T, k = ids.shape
+    out = torch.zeros((T * k, slices * n), dtype=torch.float64, device="cuda") if base is None else base.double()
+    mag, h = torch.zeros_like(out), HALF[dtype]
+    a, e = adapter.cpu().numpy().repeat(k), ids.cpu().numpy().reshape(-1)
+    for i, m in enumerate(mats):
+        if m is None:
+            continue
+        for j in range(m[0].shape[0]):
+            p = np.flatnonzero((a == i) & (e == j))
+            if not p.size:
+                continue
+            p = torch.from_numpy(p).cuda()
+            rows = x[p if per_pair else p // k].double()
+            r, sc = m[0].shape[2], float(m[2])
+            for s in range(slices):
+                A, B = m[0][j, s].double().t().contiguous(), m[1][j, s].double().t().contiguous()
+                c = slice(s * n, (s + 1) * n)
+                out[p, c] += sc * ((rows @ A) @ B)
+                mag[p, c] += abs(sc) * (2 * (K + r) * U + h * h) * ((rows.abs() @ A.abs()) @ B.abs())
+    return out, mag + 4 * U * out.abs() + h * 1.01 * out.abs() + TINY[dtype]
+
+
+def _check_grouped(got, ref, bound, adapter, ids, L, E, base):
+    err = (got.double() - ref).abs()
+    assert (err <= bound).all(), float((err / bound).max())
+    k = ids.shape[1]
+    a, e = adapter.repeat_interleave(k), ids.reshape(-1)
+    none = (a < 0) | (a >= L) | (e < 0) | (e >= E)
+    assert torch.equal(got[none], base[none] if base is not None else torch.zeros_like(got[none]))
+
+
+TILES = [
+    # K, n, slices, ranks, max_rank
+    (72, 40, 2, [16, 5], 16),
+    (1000, 264, 2, [9, 16], 16),
+    (200, 72, 2, [32, 0, 20], 32),
+    (520, 136, 1, [32, 17], 32),
+    (72, 200, 3, [32, 3], 32),
+    (200, 264, 1, [64, 33, 40], 64),
+    (1000, 40, 2, [64, 2], 64),
+    (264, 72, 1, [96, 65], 96),
+    (136, 520, 2, [128, 100, 7], 128),
+]
+
+
+@pytest.mark.parametrize("topk, per_pair, with_base", [(1, False, True), (2, False, False), (3, True, True)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("K, n, slices, ranks, max_rank", TILES)
+def test_tiles_of_64_pairs(K, n, slices, ranks, max_rank, dtype, topk, per_pair, with_base):
+    L, E = 4, 64
+    g = torch.Generator(device="cuda").manual_seed(K + n)
+    stack, mats = _stack(L, E, K, n, ranks, slices, dtype, max_rank, 5)
+    adapter, ids = _grouped_batch(L, E, topk, GROUP_SIZES, K + topk)
+    P = ids.numel()
+    assert L * E >= 256 and P > 256
+    x = torch.randn((P if per_pair else P // topk, K), generator=g, device="cuda").to(dtype)
+    base = torch.randn((P, slices * n), generator=g, device="cuda").to(dtype) if with_base else None
+    got = _lora().low_rank(x, stack, adapter, ids, base=base)
+    ref, bound = _ref_by_group(x, mats, adapter, ids, slices, n, K, base, per_pair, dtype)
+    _check_grouped(got, ref, bound, adapter, ids, L, E, base)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("K, n, slices, max_rank", [(72, 264, 1, 16), (520, 40, 3, 16), (200, 72, 1, 32)])
+def test_tiles_of_64_pairs_from_a_listing(K, n, slices, max_rank, dtype):
+    """From a listing that several projections share, whole and by an expert_map; pairs whose expert has no slot keep
+    what stood in their rows."""
+    lora, (L, E, topk) = _lora(), (4, 64, 2)
+    g = torch.Generator(device="cuda").manual_seed(K)
+    stack, mats = _stack(L, E, K, n, [max_rank, 3], slices, dtype, max_rank, 6)
+    adapter, ids = _grouped_batch(L, E, topk, GROUP_SIZES, K)
+    P = ids.numel()
+    x = torch.randn((P, K), generator=g, device="cuda").to(dtype)
+    ref, bound = _ref_by_group(x, mats, adapter, ids, slices, n, K, None, True, dtype)
+    out = torch.full((P, slices * n), 3.0, dtype=dtype, device="cuda")
+    lora.apply(x, stack, adapter, ids, P // topk, topk, True, None, out,
+               listing=lora.group(stack, adapter, ids, None, 0))
+    _check_grouped(out, ref, bound, adapter, ids, L, E, None)
+    emap = torch.arange(E, dtype=torch.int32, device="cuda") % 2 * 40 + torch.arange(E, dtype=torch.int32, device="cuda") - 8
+    slots = 50  # experts below 8 (even) have none, and those whose entry is 50 or more
+    out.fill_(3.0)
+    lora.apply(x, stack, adapter, ids, P // topk, topk, True, None, out, expert_map=emap, slots=slots,
+               listing=lora.group(stack, adapter, ids, emap, slots))
+    e = ids.reshape(-1)
+    at = emap[e.clamp(0, E - 1)]
+    routed = (e >= 0) & (e < E) & (at >= 0) & (at < slots)
+    assert routed.any() and not routed.all()
+    assert ((out.double() - ref).abs() <= bound)[routed].all()
+    assert (out[~routed] == 3).all()
+
+
+@pytest.mark.parametrize("max_rank, slices, dtype", [(32, 1, torch.float16), (16, 2, torch.bfloat16),
+                                                     (64, 1, torch.bfloat16), (128, 1, torch.float16)])
+def test_tiles_of_64_pairs_by_their_number(max_rank, slices, dtype):
+    """Few groups of thousands of pairs each, the last tile of a group in part."""
+    T, L, K, n = 16384 + 37, 3, 136, 72
+    g = torch.Generator(device="cuda").manual_seed(max_rank)
+    stack, mats = _stack(L, 1, K, n, [max_rank, 7], slices, dtype, max_rank, 8)
+    x = torch.randn((T, K), generator=g, device="cuda").to(dtype)
+    adapter = torch.randint(-1, L, (T,), generator=g, device="cuda")
+    ids = torch.zeros((T, 1), dtype=torch.int32, device="cuda")
+    got = _lora().low_rank(x, stack, adapter)
+    ref, bound = _ref_by_group(x, mats, adapter, ids, slices, n, K, None, False, dtype)
+    _check_grouped(got, ref, bound, adapter, ids, L, 1, None)
