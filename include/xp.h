@@ -614,7 +614,8 @@ int xp_router_choose_balance(const void* logits, int dtype, int64_t T,
  * through the weights (grad_weights fp32[T][topk] and the ids, nullable) and
  * through the loss (counts and tokens as written above and grad_loss, an fp32
  * scalar on the device, nullable together). The choice, the counts and the
- * bias have no gradient. Rows of padding get zeros. */
+ * bias have no gradient. An expert that stands in a row several times gets the
+ * sum of its places' terms. Rows of padding get zeros. */
 int xp_router_backward(const void* logits, int dtype, int64_t T, int64_t E,
                        int64_t row_stride, int64_t topk, int scoring,
                        int renormalize, double scale, const uint8_t* mask,

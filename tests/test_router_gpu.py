@@ -634,3 +634,66 @@ def test_balance_of_every_form(T, E, k, dtype, how, cuts):
     bound = _grad_bound(ref, near, reach, E, dtype)
     assert (err <= bound).all(), float((err / bound).max())
     assert (grad.cpu()[~torch.from_numpy(live_rows)] == 0).all()
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("E, k, dtype", [(60, 4, torch.float32), (256, 16, torch.bfloat16), (12, 8, torch.float16),
+                                         (600, 5, torch.float32), (40, 20, torch.float32)])
+def test_gradient_of_repeated_ids(E, k, dtype, scoring, renorm):
+    """The C entry point takes any choice: an expert that stands in a row several times gets the sum of its terms,
+    through the weights and the loss together, in both forms of the rows."""
+    from vllm_expert_pager import _native as nat
+
+    T, scale, gl = 70, 2.5, 512.0
+    g = np.random.default_rng(E + k)
+    logits = _logits(T, E, dtype, E - k)
+    ids = np.stack([g.permutation(E)[np.arange(k) % (E // 2 + 1)] for _ in range(T)])
+    ids[:, k - 1] = ids[:, 0]  # the first and the last place of every row
+    ids[3] = ids[3, 0]
+    ids[4, 1:] = -1
+    ids[5] = -1
+    if k > 4:
+        ids[6::5, 1:4] = ids[6::5, 2:3]
+    ids = ids.astype(np.int32)
+    gw = torch.randn((T, k), generator=torch.Generator().manual_seed(3))
+    z = logits.double().numpy()
+    on = np.ones(T, bool)
+    _, counts, spread = _balance_ref(z, ids, k, scoring, on, [0, T])
+    dev = [torch.from_numpy(ids).cuda(), gw.cuda(), torch.from_numpy(counts.astype(np.int32)).cuda(),
+           torch.tensor([T, 1], dtype=torch.int32, device="cuda"), torch.tensor(gl, device="cuda")]
+    leaf = logits.cuda()
+    grad = torch.full((T, E), 7.0, dtype=dtype, device="cuda")
+    _router()  # (the library's path)
+    nat.call_on(leaf, "xp_router_backward", leaf.data_ptr(), {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype],
+                T, E, E, k, 1 if scoring == "sigmoid" else 0, renorm, scale, None, None, 1, dev[0].data_ptr(), 4,
+                dev[1].data_ptr(), dev[2].data_ptr(), dev[3].data_ptr(), dev[4].data_ptr(), grad.data_ptr())
+    score, p = _score(z, scoring)
+    rows = np.arange(T)[:, None]
+    live = ids >= 0
+    at = np.where(live, ids, 0)
+    own = np.where(live, score[rows, at], 0.0)
+    g64 = np.where(live, gw.double().numpy() * scale, 0.0)
+    slope = 1 - score[rows, at] if scoring == "sigmoid" else np.ones((T, k))
+    if renorm:
+        own = own / np.maximum(own.sum(1, keepdims=True), 1e-300)
+        term = own * slope * (g64 - (g64 * own).sum(1, keepdims=True))
+    elif scoring == "sigmoid":
+        term = g64 * own * slope
+    ref, near, full = gl * spread, p.copy(), np.zeros((T, E))
+    for t in range(T):
+        for j in range(k):
+            if not live[t, j]:
+                continue
+            near[t, at[t, j]] += own[t, j]
+            if renorm or scoring == "sigmoid":
+                ref[t, at[t, j]] += term[t, j]
+            else:
+                full[t, at[t, j]] += g64[t, j]
+    if not renorm and scoring == "softmax":
+        ref = ref + p * (full - (full * p).sum(1, keepdims=True))
+    # _grad_bound with every place's terms in the reach: k of them add up where an expert repeats.
+    reach = np.abs(g64).sum(1, keepdims=True) + gl * counts.max() * E / (k * T * T)
+    err = np.abs(grad.double().cpu().numpy() - ref)
+    bound = _grad_bound(ref, near, reach, E, dtype)
+    assert (err <= bound).all(), float((err / bound).max())
