@@ -697,3 +697,19 @@ def test_gradient_of_repeated_ids(E, k, dtype, scoring, renorm):
     err = np.abs(grad.double().cpu().numpy() - ref)
     bound = _grad_bound(ref, near, reach, E, dtype)
     assert (err <= bound).all(), float((err / bound).max())
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor's tangent is never dropped in silence: the calls have no forward mode and say so."""
+    router = _router()
+    fw = torch.autograd.forward_ad
+    z = _logits(6, 16, torch.float32, 2).cuda()
+    want = router.choose_experts(z, 2)
+    with fw.dual_level():
+        dual = fw.make_dual(z, torch.ones_like(z))
+        for call in (lambda: router.choose_experts(dual, 2), lambda: router.choose_and_balance(dual, 2),
+                     lambda: router.balance_loss(dual, want[1])):
+            with pytest.raises(NotImplementedError):
+                call()
+        got = router.choose_experts(z, 2)  # a tensor without a tangent
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -21,6 +21,7 @@ results with torch and can be captured in a graph.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from vllm_expert_pager import _native as nat
 
@@ -224,7 +225,8 @@ def choose_experts(
     logits = _logits(logits)
     bias = _pick(logits, topk, bias, groups, topk_groups)
     args = (logits, topk, code, bool(renormalize), bias, groups, topk_groups, float(scale), _mask(mask, logits))
-    if logits.requires_grad and torch.is_grad_enabled():
+    # Inside a level of forward mode the function is taken as well: it refuses a tensor that carries a tangent.
+    if (logits.requires_grad and torch.is_grad_enabled()) or getattr(forward_ad, "_current_level", 0) >= 0:
         return _Choose.apply(*args)
     return _choose(*args)  # serving: no graph, and none of its cost (a third of a one-token call's host time)
 
