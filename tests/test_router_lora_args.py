@@ -163,3 +163,10 @@ def test_expert_map_of_an_adapted_chunk(bad):
     batch = lora.AdaptedBatch(lora.ExpertAdapters(down=stack), ids[:, 0].contiguous(), ids, None, None)
     with pytest.raises(ValueError, match="expert_map"):
         batch.down(torch.zeros((6, 16), dtype=torch.bfloat16), bad, 8)
+
+
+@pytest.mark.parametrize("T, E, topk", [((1 << 28) + 1, 8, 2), ((1 << 26) + 1, 600, 2), ((1 << 31) - 1, 1, 1)])
+def test_more_rows_than_a_launch_has_threads_for(T, E, topk):
+    for name, args in (("xp_router_choose", CHOOSE), ("xp_router_backward", BACK)):
+        with pytest.raises(nat.NativeError, match="launch grid"):
+            nat.call(name, *{**args, "T": T, "E": E, "stride": E, "topk": topk}.values())

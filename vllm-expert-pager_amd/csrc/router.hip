@@ -1318,6 +1318,15 @@ int balance_parts(int64_t T, int64_t num_seqs) {
   return static_cast<int>(std::max<int64_t>(parts, 1));
 }
 
+// The grid of a launch of `per_block` rows a workgroup: fewer than 2^32 threads.
+int row_grid(const Call& c, int per_block, dim3* grid) {
+  const int64_t blocks = (c.T + per_block - 1) / per_block;
+  if (blocks * kThreads > UINT32_MAX)
+    return fail(XP_E_LIMIT, "%s: %lld rows exceed the launch grid", c.what, (long long)c.T);
+  *grid = dim3(static_cast<unsigned>(blocks));
+  return XP_OK;
+}
+
 int64_t align256(int64_t n) { return (n + 255) & ~int64_t(255); }
 
 int64_t join_blocks(int64_t E) { return (E + kJoinExperts - 1) / kJoinExperts; }
@@ -1394,7 +1403,8 @@ int xp_router_choose(const void* logits, int dtype, int64_t T, int64_t E, int64_
   const int lanes = narrow ? kRowLanes : 64, per_block = narrow ? kBlockRows : kWaves;
   const Rows r = rows_of(c, lanes);
   const size_t lds = groups > 1 ? static_cast<size_t>(kWaves) * E * (bias ? 8 : 4) : 0;
-  const dim3 grid(static_cast<unsigned>((T + per_block - 1) / per_block));
+  dim3 grid;
+  if (int rc = row_grid(c, per_block, &grid)) return rc;
   dispatch(dtype, values_per_lane(E, lanes), [&](auto type, auto v) {
     using L = decltype(type);
     constexpr int V = decltype(v)::value;
@@ -1478,7 +1488,8 @@ int xp_router_backward(const void* logits, int dtype, int64_t T, int64_t E, int6
   const bool narrow = narrow_rows(E, topk);
   const int lanes = narrow ? kRowLanes : 64, per_block = narrow ? kBlockRows : kWaves;
   const Rows r = rows_of(c, lanes);
-  const dim3 grid(static_cast<unsigned>((T + per_block - 1) / per_block));
+  dim3 grid;
+  if (int rc = row_grid(c, per_block, &grid)) return rc;
   dispatch(dtype, values_per_lane(E, lanes), [&](auto type, auto v) {
     using L = decltype(type);
     constexpr int V = decltype(v)::value;
