@@ -45,7 +45,6 @@ namespace xp {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -109,7 +108,6 @@ struct Ids {
   int slots;
   int adapters, experts;
   Divisor by_topk, by_experts;
-  int64_t topk;
 };
 
 // Pair p's group: adapter * experts + expert, adapters * experts for a pair
@@ -797,7 +795,7 @@ int check_ids(const char* what, const void* adapter_ids, int aeb, const void* to
   XP_REQUIRE(expert_map == nullptr || (slots >= 0 && slots <= INT32_MAX), "%s: %lld slots", what, (long long)slots);
   XP_REQUIRE(T == 0 || adapter_ids, "%s: null adapter ids", what);
   *d = Ids{adapter_ids, topk_ids, aeb, eb, expert_map, static_cast<int>(slots),
-           static_cast<int>(adapters), static_cast<int>(experts), divisor(topk), divisor(experts), topk};
+           static_cast<int>(adapters), static_cast<int>(experts), divisor(topk), divisor(experts)};
   return XP_OK;
 }
 
