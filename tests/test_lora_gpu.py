@@ -313,9 +313,9 @@ def test_offsets_past_32_bits():
     assert y[: T - tail].abs().max() == 0 and own[who[-tail:] >= 0].abs().sum() > 0
 
 
-# Tiles of 64 pairs: listings of 256 groups or of 16384 pairs at least. A call of one slice (or three) of rank 16 that
-# lists for itself takes 16-pair tiles instead, the large cases of test_any_order_and_any_split among them; from a
-# listing of lora.group it gets tiles of 64 too.
+# Tiles of 64 pairs: listings of 256 groups or of 16384 pairs at least. A call that lists for itself takes 16-pair tiles
+# instead where it has one slice (or three) of rank 16, the large cases of test_any_order_and_any_split among them, or
+# rank 96 or 128; from a listing of lora.group it gets tiles of 64 too.
 
 GROUP_SIZES = [1, 16, 17, 33, 63, 64, 65, 130]
 
@@ -405,7 +405,8 @@ def test_tiles_of_64_pairs(K, n, slices, ranks, max_rank, dtype, topk, per_pair,
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("K, n, slices, max_rank", [(72, 264, 1, 16), (520, 40, 3, 16), (200, 72, 1, 32)])
+@pytest.mark.parametrize("K, n, slices, max_rank", [(72, 264, 1, 16), (520, 40, 3, 16), (200, 72, 1, 32),
+                                                        (264, 72, 1, 96), (136, 520, 2, 128)])
 def test_tiles_of_64_pairs_from_a_listing(K, n, slices, max_rank, dtype):
     """From a listing that several projections share, whole and by an expert_map; pairs whose expert has no slot keep
     what stood in their rows."""

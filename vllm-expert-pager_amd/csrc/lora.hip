@@ -738,11 +738,17 @@ int tile_pairs(int64_t npairs, int64_t adapters, int64_t experts) {
 // single slice of rank 16 gains little from 64 (16 rows of A are soon read) and
 // loses the workgroups. us with 64 and with 16, 256 experts x 8 and four
 // adapters: K = 512, 2048 and 4096, 2048 tokens 46 and 41, 76 and 64, 105 and 86,
-// 8192 tokens 122 and 117, 166 and 160, 223 and 208; 32768 dense tokens of 16
-// adapters 84 and 76, of one 77 and 88. With rank 32 (K = 512, 8192 tokens) 136
-// and 177, dense 96 and 111; rank 64 dense 135 and 191.
+// 8192 tokens 122 and 117, 166 and 160, 223 and 208; 32768 dense tokens (2048 x
+// 2048) of 16 adapters 84 and 76, of one 77 and 88. With rank 32 (K = 512, 8192
+// tokens) 136 and 177, dense 96 and 111; rank 64 dense 135 and 191.
+// Ranks 96 and 128 have no shape of more than 16 pairs at a time (pick_shape), so
+// a tile of 64 reads A and B as often as four of 16, in a quarter of the
+// workgroups: down of 2048 tokens with two adapters 160 and 105, 215 and 138, of
+// 8192 with one 276 and 263, 421 and 365; gate and up of 8192 tokens x 4 of 64
+// experts 211 and 169, 317 and 265; 32768 dense tokens of 16 adapters 219 and 177,
+// 350 and 264, of one 151 and 153, 226 and 234.
 int own_tile_pairs(int64_t npairs, int64_t adapters, int64_t experts, int64_t slices, int64_t R) {
-  return R == 16 && slices % 2 == 1 ? kFrag : tile_pairs(npairs, adapters, experts);
+  return R >= 96 || (R == 16 && slices % 2 == 1) ? kFrag : tile_pairs(npairs, adapters, experts);
 }
 
 // Workgroups that a call of few tiles is split into, about. Every part of a
