@@ -660,10 +660,11 @@ int xp_lora_group(const void* adapter_ids, int adapter_elem_bytes,
  * expert e, row = t, or p with per_pair; one rounding to the type of out. A
  * pair without an adapter gets base. base null: 0. Rows are x_stride,
  * base_stride and out_stride elements apart (multiples of 8); out may be
- * base, with the same stride. Sums and the inner product in fp32 (the inner product enters the
- * second one as a sum of two values of the type). grouped != 0: the workspace
- * holds the listing of xp_lora_group for the same ids and sizes; else the call
- * makes it. Calls of at most 256 pairs group themselves and need no workspace. */
+ * base, with the same stride. Sums and the inner product in fp32 (the inner
+ * product enters the second one as a sum of two values of the type). grouped
+ * != 0: the workspace holds the listing of xp_lora_group for the same ids and
+ * sizes; else the call makes it. Calls of at most 256 pairs group themselves
+ * and need no workspace. */
 int xp_lora_apply(const void* x, int dtype, int64_t x_stride, int per_pair,
                   int64_t T, int64_t topk, int64_t K, const void* a,
                   const void* b, const float* scales, const int32_t* ranks,

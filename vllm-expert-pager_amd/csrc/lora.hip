@@ -16,8 +16,12 @@
 // Few tiles (decode steps): a workgroup per tile, slice and part of the
 // columns, each of which makes u for itself from a matrix A that the parts
 // read out of one L2 (64 dense tokens, rank 64: 13.7 us). Many tiles: a workgroup
-// per tile of 64 pairs takes both slices, so that A, B and x are read once (gate
-// and up of 8192 tokens x 8: 117 us, 617 MB at 5.2 TB/s).
+// per tile of 64 pairs, as many of them at a time as its registers hold (MT
+// fragments), and both slices of an even number where the rank is at most 32. A
+// and B are read once for the tile at rank 16 and, for one slice, 32; twice at 64
+// and for two slices of 32; at 96 and 128 once per 16 pairs. x is read once for
+// the slices that go together (gate and up of 8192 tokens x 8, rank 16: 117 us,
+// 617 MB at 5.2 TB/s).
 //
 // u enters the second product as the sum of two values of the operands' type,
 // its rounding and the rounding of what is left, so no more than 2^-16 of it

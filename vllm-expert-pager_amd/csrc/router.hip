@@ -27,9 +27,10 @@
 // on the one before it for long. Otherwise a row is a wave's, and the choice a
 // round per expert: the largest key of all lanes, its first holder, and that
 // key taken out. 32768 tokens of 256 experts, top-8, bf16, choice and loss: 18 us
-// by the first form, 62 by the second; their backward 13.5 and 29. Bound there
-// by VALU instructions (1.1 and 2.6 TB/s); 4096 tokens in 8 groups with a bias,
-// 13 us, by the rounds; below some hundred tokens by a launch's latency (2.7 us).
+// by the first form, 62 by the second; their backward 13.5 and 29 (other sizes at
+// narrow_rows). Bound there by VALU instructions (1.1 and 2.6 TB/s); 4096 tokens
+// in 8 groups with a bias, 13 us, by the rounds; below some hundred tokens by a
+// launch's latency (2.7 us).
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
@@ -1276,7 +1277,17 @@ int values_per_lane(int64_t E, int lanes) {
   return v;
 }
 
-// Whether rows are 16 lanes' (see the top).
+// Whether rows are 16 lanes' (see the top). us in a graph by that form and by a
+// wave per row, 32768 tokens, choice alone | choice and loss | with the backward:
+//   8 experts, top-2, bf16             5.0 and 9.7 | 12 and 28 | 17 and 42
+//   256 experts, top-16, fp32          17 and 39 | 30 and 92 | 50 and 126
+//   512 experts, top-10, bf16          20 and 35 | 37 and 91 | 63 and 145
+//   512 experts, top-16, fp32          25 and 50 | 42 and 118 | 84 and 203
+//   the same by the sigmoid            25 and 53 | 59 and 150 | 106 and 225
+// At 64 tokens the choice alone is the slower one for some (64 experts, fp32, 3.2
+// and 2.8; 384, whose lanes do not share them evenly, 6.0 and 5.0), with the loss
+// none is (8.4 and 11.3; 13.2 and 22.6). Beyond the rule: 1024 experts, top-8, 44 |
+// 111 | 249 for 32768 tokens; 256 experts, top-33, 70 | 157 | 203.
 bool narrow_rows(int64_t E, int64_t topk) { return E <= kNarrowExperts && topk <= kNarrowTopk; }
 
 Rows rows_of(const Call& c, int lanes) {
@@ -1311,7 +1322,11 @@ void dispatch(int dtype, int vpl, F&& f) {
 }
 
 // Workgroups that share a sequence: kBlockRows rows each at least, and no more
-// than about 512 in all (the join reads a row of E sums from each).
+// than about 512 in all (the join reads a row of E sums from each). Every
+// sequence gets as many, by their average length: one that holds most of the
+// rows is done by its own few, and its sums run over as many more rows each
+// (choice and loss of 32768 tokens, 256 experts: 40 even sequences 37 us, one of
+// 32000 rows among 40 344; 512 even ones 209, one of 32000 rows among 512 4020).
 int balance_parts(int64_t T, int64_t num_seqs) {
   const int64_t per = (T + num_seqs - 1) / num_seqs;
   const int64_t parts = std::min<int64_t>((per + kBlockRows - 1) / kBlockRows, std::max<int64_t>(1, 512 / num_seqs));

@@ -72,7 +72,8 @@ class LowRankAdapters:
     def load(self, adapter: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
         """Put an adapter in place: ``a`` ``(experts, slices, r, in_features)`` and ``b`` ``(experts, slices,
         out_features / slices, r)``; without the slices' dimension for one slice, without the experts' for one
-        expert. ``scale`` multiplies its output (alpha / r). On the current stream, as any other copy."""
+        expert. ``scale`` multiplies its output (alpha / r). On the current stream, as any other copy; bringing A
+        into the kernels' order costs up to as much again as copying both."""
         self._index(adapter)
         lead = (self.experts, self.slices)
         # What may stand before a matrix: both dimensions, or without one (or both) of size 1.

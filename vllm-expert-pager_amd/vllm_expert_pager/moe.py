@@ -375,7 +375,8 @@ def fused_moe(
     Without ``expert_map`` the slab holds every expert (slot e = expert e).
     Pairs whose expert has no slot contribute nothing. ``adapters`` add the
     low-rank adapters of the requests, token t's being ``adapter_ids[t]`` (-1:
-    none; such a token gets the bits of a call without adapters).
+    none; such a token gets the bits of a call without adapters). The result
+    carries no gradient, by tokens, weights or adapters.
     """
     S = w13.shape[0]
     E = num_experts if num_experts is not None else (expert_map.numel() if expert_map is not None else S)

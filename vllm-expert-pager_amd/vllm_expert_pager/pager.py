@@ -226,7 +226,8 @@ class PagedExperts:
         ``adapters`` add the requests' low-rank adapters beside the layer's
         experts, token t's being ``adapter_ids[t]`` (-1: none). They are
         addressed by expert id and stay in HBM, so they take no part in the
-        paging; the reference has no counterpart.
+        paging; the reference has no counterpart. The output carries no
+        gradient.
         """
         if not self.ready:
             raise RuntimeError(f"layer {self.layer}: setup() has not run")

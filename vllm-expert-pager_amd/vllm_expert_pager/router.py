@@ -13,8 +13,11 @@ as they are: an id of -1 (a padded token, or fewer experts left than topk) adds
 nothing there. ``counts`` tell which experts a traffic prefers, which decides
 the tables' hit rates; the loss trains a router towards or away from it.
 
-The weights and the loss are differentiable by the logits; ids and counts are
-not. All calls run on the current stream of the logits' device, allocate their
+The weights and the loss are differentiable by the logits (backward, first
+order); ids and counts are not. The expert calls of this package return tensors
+without a graph: a gradient of ``topk_weights`` comes from experts that are run
+elsewhere, and beside frozen experts served here a router is trained by the loss
+alone. All calls run on the current stream of the logits' device, allocate their
 results with torch and can be captured in a graph.
 """
 
@@ -220,6 +223,7 @@ def choose_experts(
     ``topk_groups`` best groups of ``E / groups`` consecutive experts are
     chosen from: by their best expert, or with a bias by the sum of their best
     two. ``mask`` (bool, ``(T,)``): False marks padding, whose ids are -1.
+    At most 2048 experts, 64 chosen, and 64 groups (of at most 1024 experts).
     """
     code = _scoring(scoring)
     logits = _logits(logits)
@@ -248,7 +252,8 @@ def balance_loss(
     ``(B + 1,)``) sequence s holds the rows ``[seq_offsets[s],
     seq_offsets[s + 1])``, counts are ``(B, E)``, and the loss is the mean over
     the sequences that have tokens; rows outside of all are padding. Padding,
-    and ids outside ``[0, E)``, count nowhere.
+    and ids outside ``[0, E)``, count nowhere. Every sequence is given the same
+    number of workgroups, so lengths of one order are summed fastest.
     """
     code = _scoring(scoring)
     logits = _logits(logits)
